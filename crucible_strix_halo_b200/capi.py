@@ -9,6 +9,7 @@ OK, ERR_INVALID, ERR_CUDA, ERR_UNSUPPORTED, ERR_TIMEOUT = range(5)
 OUT_RAW_F32, OUT_RAW_BF16, OUT_EXL3_WHT = range(3)
 IN_F32, IN_BF16 = range(2)
 GDN_SERIAL_F32, GDN_CHUNK_TC = range(2)
+ROW_F32, ROW_BF16, ROW_F16 = range(3)
 PEND_FLOATS, QSA_PART, QSA_SPLITS, SEL_BLOCKS, MAX_STEP_ROWS = 258, 258, 32, 512, 13
 
 
@@ -43,6 +44,16 @@ class Span(C.Structure):
 
 class ProjOut(C.Structure):
     _fields_ = [("ptr", P), ("col0", C.c_int), ("cols", C.c_int), ("ld", C.c_int), ("f32", C.c_int)]
+
+
+class Mx4(C.Structure):
+    _fields_ = [("codes", P), ("scales", P), ("rows", C.c_int), ("inner", C.c_int)]
+
+
+class LogitsArgs(C.Structure):
+    _fields_ = [("logits", P), ("out", P), ("choice", P), ("counts", P), ("drafts", P), ("bias", P), ("mask", P), ("ld", C.c_longlong),
+                ("out_ld", C.c_longlong), ("mask_ld", C.c_longlong), ("R", C.c_int), ("V", C.c_int), ("dtype", C.c_int),
+                ("repetition", C.c_float), ("frequency", C.c_float), ("presence", C.c_float)]
 
 
 class GdnArgs(C.Structure):
@@ -117,6 +128,14 @@ _protos = {
     "cr_qsa_shard_attn": (C.c_int, [G, C.POINTER(QsaArgs), C.c_int, C.c_int, P, P, C.c_size_t, P]),
     "cr_qsa_merge_partials": (C.c_int, [G, C.POINTER(QsaArgs), C.c_int, P, C.c_int, P]),
     "cr_proj_gemm": (C.c_int, [P, P, C.c_int, C.c_int, C.c_int, C.POINTER(ProjOut), C.c_int, P]),
+    "cr_mx4_code_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "cr_mx4_scale_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "cr_mx4_quant": (C.c_int, [P, C.c_int, C.c_longlong, C.POINTER(Mx4), P]),
+    "cr_mx4_dequant": (C.c_int, [C.POINTER(Mx4), P, C.c_int, C.c_longlong, P]),
+    "cr_mx4_gemm": (C.c_int, [C.POINTER(Mx4), C.POINTER(Mx4), C.POINTER(ProjOut), C.c_int, P]),
+    "cr_mx4_rows": (C.c_int, [P, C.c_int, C.c_longlong, C.c_int, C.POINTER(Mx4), C.POINTER(ProjOut), C.c_int, P]),
+    "cr_logits_choose": (C.c_int, [C.POINTER(LogitsArgs), C.c_int, P]),
+    "cr_token_count": (C.c_int, [P, C.c_int, C.c_int, P, C.c_int, P]),
     "cr_spans_bytes": (C.c_size_t, [C.POINTER(Span), C.c_int]),
     "cr_state_save": (C.c_int, [C.POINTER(Span), C.c_int, P, C.c_size_t, P]),
     "cr_state_restore": (C.c_int, [C.POINTER(Span), C.c_int, P, C.c_size_t, P]),

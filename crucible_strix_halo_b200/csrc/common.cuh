@@ -10,6 +10,7 @@
 
 #include <atomic>
 #include <mutex>
+#include <type_traits>
 #include <utility>
 #include <cstdlib>
 

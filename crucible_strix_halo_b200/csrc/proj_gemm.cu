@@ -26,9 +26,7 @@
 // the matrix are zero-filled by the copy engine and masked in the epilogue.  Every wait is bounded; a wait that gives up
 // raises bit 4 of the device status word.
 #include <cooperative_groups.h>
-#include "common.cuh"
-#include "tma.cuh"
-#include "umma.cuh"
+#include "proj.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -38,70 +36,11 @@ CR_DEFINE_STATUS_WORD(proj_gemm)
 
 constexpr int kGM = 128, kGK = 64;
 constexpr int kGThreads = 192;
-constexpr int kMaxOuts = 6;
 constexpr int kTileBytes = kGM * kGK * 2;                       // 128 rows x 64 channels of X or W
 
-struct ProjParams {
-  int R, K, N, n_outs;
-  void* ptr[kMaxOuts];
-  int col0[kMaxOuts], cols[kMaxOuts], ld[kMaxOuts], f32[kMaxOuts];
-};
-
-__device__ __forceinline__ void load_box_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(
-                   umma::smem_u32(dst)),
-               "l"(map), "r"(c0), "r"(c1), "r"(umma::smem_u32(bar))
-               : "memory");
-}
 // Instruction descriptor for kind::f16 with bf16 operands (format 1), fp32 accumulation, both operands K-major.
 __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-
-// ---- CTA pairs: the cta_group::2 forms --------------------------------------------------------------------------
-// A box into this CTA's shared memory whose bytes complete on a barrier of either CTA of the pair.
-__device__ __forceinline__ void pair_load_box_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];\n" ::"r"(
-                   umma::smem_u32(dst)),
-               "l"(map), "r"(c0), "r"(c1), "r"(bar)
-               : "memory");
-}
-__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory"); }
-
-// Columns col .. col + 31 of one row to the output that owns them.
-__device__ __forceinline__ void store_chunk(const ProjParams& P, int row, int col, const float (&v)[32]) {
-  int o = 0;
-  while (o < P.n_outs - 1 && col >= P.col0[o] + P.cols[o]) ++o;       // outputs are ordered by column; chunks do not straddle them
-  const size_t at = (size_t)row * P.ld[o] + (col - P.col0[o]);
-  if (P.f32[o]) {
-    float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(P.ptr[o]) + at);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) dst[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-  } else {
-    uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(P.ptr[o]) + at);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      unsigned pk[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const __nv_bfloat162 b2 = __floats2bfloat162_rn(v[8 * k + 2 * j], v[8 * k + 2 * j + 1]);
-        pk[j] = *reinterpret_cast<const unsigned*>(&b2);
-      }
-      dst[k] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-    }
-  }
-}
-// Four columns of one row.
-__device__ __forceinline__ void store_quad(const ProjParams& P, int row, int col, const float4 v) {
-  int o = 0;
-  while (o < P.n_outs - 1 && col >= P.col0[o] + P.cols[o]) ++o;
-  const size_t at = (size_t)row * P.ld[o] + (col - P.col0[o]);
-  if (P.f32[o]) *reinterpret_cast<float4*>(reinterpret_cast<float*>(P.ptr[o]) + at) = v;
-  else {
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
-    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(P.ptr[o]) + at) =
-        make_uint2(*reinterpret_cast<const unsigned*>(&lo), *reinterpret_cast<const unsigned*>(&hi));
-  }
 }
 
 // ---- CTA pairs on 256 x 256 tiles ----------------------------------------------------------------------------------
@@ -447,19 +386,9 @@ extern "C" cr_status cr_proj_gemm(const void* x, const void* w, int R, int K, in
   using namespace cr;
   CR_REQUIRE(x && w && outs, "cr_proj_gemm: null buffer");
   CR_REQUIRE(R >= 1 && N >= 32 && K >= kGK && K % kGK == 0, "cr_proj_gemm: R >= 1, N >= 32, K a multiple of 64 (got R=%d K=%d N=%d)", R, K, N);
-  CR_REQUIRE(n_outs >= 1 && n_outs <= kMaxOuts, "cr_proj_gemm: 1..%d outputs", kMaxOuts);
   CR_REQUIRE(((uintptr_t)x & 15) == 0 && ((uintptr_t)w & 15) == 0, "cr_proj_gemm: operands must be 16-byte aligned");
   ProjParams P;
-  P.R = R; P.K = K; P.N = N; P.n_outs = n_outs;
-  int next = 0;
-  for (int i = 0; i < n_outs; ++i) {
-    const cr_proj_out& o = outs[i];
-    CR_REQUIRE(o.ptr && o.col0 == next && o.cols >= 32 && o.cols % 32 == 0, "cr_proj_gemm: output %d must start at column %d and hold a multiple of 32 columns", i, next);
-    CR_REQUIRE(o.ld >= o.cols && (o.ld * (o.f32 ? 4 : 2)) % 16 == 0 && ((uintptr_t)o.ptr & 15) == 0, "cr_proj_gemm: output %d: row pitch and base must keep 16-byte alignment", i);
-    P.ptr[i] = o.ptr; P.col0[i] = o.col0; P.cols[i] = o.cols; P.ld[i] = o.ld; P.f32[i] = o.f32 ? 1 : 0;
-    next += o.cols;
-  }
-  CR_REQUIRE(next == N, "cr_proj_gemm: the outputs cover %d columns, the product has %d", next, N);
+  if (cr_status st = list_outs(P, "cr_proj_gemm", R, K, N, outs, n_outs)) return st;
   const int(*slots)[9];
   if (cr_status st = cluster_slots(&slots)) return st;
   const GemmShape shape = gemm_shape(R, K, N, sm_count(), *slots);

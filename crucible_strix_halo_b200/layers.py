@@ -174,3 +174,58 @@ def proj_gemm(x, w, outs):
     """x [R, K] bf16, w [N, K] bf16 (out x in); outs: list of (tensor [R, cols] bf16 or fp32, contiguous rows) whose
     widths add up to N.  One cr_proj_gemm launch (the input or output GEMM group of a prefill layer)."""
     return _binding.proj_gemm(x, w, outs)
+
+
+class Mx4:
+    """A matrix [rows][inner] of microscaled 4-bit floats (cr_mx4): codes, uint8 [rows, inner / 2], and scales, uint8 in tiles of
+    128 rows x 4 blocks of 32 elements.  inner is a multiple of 64."""
+    __slots__ = ("codes", "scales", "rows", "inner")
+
+    def __init__(self, codes, scales, rows, inner):
+        self.codes, self.scales, self.rows, self.inner = codes, scales, rows, inner
+
+    @classmethod
+    def empty(cls, rows, inner, device="cuda"):
+        if rows < 1 or inner < 64 or inner % 64:
+            raise ValueError("a 4-bit matrix has at least one row and a multiple of 64 elements in it")
+        return cls(torch.empty(rows, inner // 2, device=device, dtype=torch.uint8),
+                   torch.empty((rows + 127) // 128 * ((inner + 127) // 128) * 512, device=device, dtype=torch.uint8), rows, inner)
+
+
+def mx4_quant(x, out=None):
+    """Rows x [rows, inner] (float32, bfloat16 or float16, any row pitch) as an Mx4 (cr_mx4_quant)."""
+    if out is None:
+        if x.dim() != 2:
+            raise ValueError("x must be a matrix")
+        out = Mx4.empty(x.shape[0], x.shape[1], x.device)
+    return _binding.mx4_quant(x, out)
+
+
+def mx4_dequant(m, dtype=torch.float32, out=None):
+    """The numbers an Mx4 stands for, as rows of `dtype` (cr_mx4_dequant)."""
+    return _binding.mx4_dequant(m, torch.empty(m.rows, m.inner, device=m.codes.device, dtype=dtype) if out is None else out)
+
+
+def mx4_gemm(x, w, outs):
+    """x, w: Mx4 of [R, K] and [N, K]; outs: list of matrices [R, cols], float32 or bfloat16, whose widths (multiples of 32) add up
+    to N.  One cr_mx4_gemm launch: the projections of a prompt's rows."""
+    return _binding.mx4_gemm(x, w, outs)
+
+
+def mx4_rows(x, w, outs):
+    """The same product with x [R, K] as it is, float32, bfloat16 or float16 (cr_mx4_rows): the projections of decode and verify
+    rows, and the head."""
+    return _binding.mx4_rows(x, w, outs)
+
+
+def logits_choose(spans, outs=None):
+    """spans: list of dicts(logits [R, V] float32 / bfloat16 / float16; and, each optional: counts int32 [V], drafts int32 [R - 1], bias
+    float32 [V], mask int32 words [ceil(V / 32)] or [R, ceil(V / 32)], repetition, frequency, presence, out float32 [R, V] for the
+    processed logits, the logits themselves included).  Penalties, bias, mask and the greedy choice of every span (cr_logits_choose);
+    returns the choices, int32 [R] each, -1 where nothing is allowed."""
+    return _binding.logits_choose(spans, outs)
+
+
+def token_count(counts, tokens, delta=1):
+    """counts int32 [V] += delta for every token of `tokens` (int32) (cr_token_count)."""
+    return _binding.token_count(counts, tokens, delta)

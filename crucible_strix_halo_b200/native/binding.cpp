@@ -9,13 +9,23 @@
 #include <vector>
 #include "../../include/crucible_attn.h"
 
+// The binding also loads beside a library that has the core's entry points alone: these may be missing there, and calling them
+// is an error then.
+#pragma weak cr_mx4_quant
+#pragma weak cr_mx4_dequant
+#pragma weak cr_mx4_gemm
+#pragma weak cr_mx4_rows
+#pragma weak cr_logits_choose
+#pragma weak cr_token_count
+
 namespace {
 
 // ---- names, interned once ---------------------------------------------------------------------------------------
 #define NAMES(X)                                                                                                        \
   X(g) X(conv) X(A_log) X(dt_bias) X(gamma) X(ab) X(suh) X(state) X(hist) X(pend) X(pend_rows) X(session) X(qkv) X(z) X(x) X(pos0) \
   X(replay) X(commit) X(q) X(k) X(v) X(idx) X(q_norm1) X(k_norm1) X(iq_norm1) X(ik_norm1) X(rope) X(ik_raw) X(ik_pool) X(raw_slots) \
-  X(scores) X(sstride) X(sel) X(nsel) X(w) X(fmt) X(scratch) X(workspace) X(out) X(raw_y) X(in_dtype) X(q_hi) X(data_ptr)
+  X(scores) X(sstride) X(sel) X(nsel) X(w) X(fmt) X(scratch) X(workspace) X(out) X(raw_y) X(in_dtype) X(q_hi) X(data_ptr) \
+  X(codes) X(scales) X(rows) X(inner) X(logits) X(counts) X(drafts) X(bias) X(mask) X(repetition) X(frequency) X(presence)
 #define DECLARE(n) PyObject* s_##n;
 NAMES(DECLARE)
 
@@ -302,6 +312,222 @@ PyObject* proj_gemm(PyObject*, PyObject* args) {     // (x, w, outs)
   });
 }
 
+// ---- 4-bit projections and the choice of a token --------------------------------------------------------------------
+// These take tensors of several types and strides, so they look at what they are given.
+[[noreturn]] void refuse(PyObject* type, const char* fmt, const char* what) { PyErr_Format(type, fmt, what); throw Error(); }
+template <typename F>
+F* present(F* f) {
+  if (!f) refuse(PyExc_RuntimeError, "%s", "the library beside this binding lacks the entry point");
+  return f;
+}
+// A tensor on the current device.
+const at::Tensor& here(PyObject* o, const char* what) {
+  const at::Tensor& t = tensor(o);
+  if (!t.is_cuda()) refuse(PyExc_ValueError, "%s must be a CUDA tensor", what);
+  if (t.get_device() != c10::cuda::current_device()) refuse(PyExc_ValueError, "%s is on another device than the current one", what);
+  return t;
+}
+cr_row_dtype row_type(const at::Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return CR_ROW_F32;
+    case at::kBFloat16: return CR_ROW_BF16;
+    case at::kHalf: return CR_ROW_F16;
+    default: refuse(PyExc_TypeError, "%s must be float32, bfloat16 or float16", what);
+  }
+}
+// Rows whose elements lie side by side; the pitch between rows.  (Of a single row any pitch will do.)
+int64_t pitch(const at::Tensor& t, const char* what) {
+  if (t.dim() != 2) refuse(PyExc_ValueError, "%s must be a matrix", what);
+  if (t.size(1) > 1 && t.stride(1) != 1) refuse(PyExc_ValueError, "%s must have its elements of a row side by side", what);
+  if (t.size(0) <= 1) return t.size(1);
+  if (t.stride(0) < t.size(1)) refuse(PyExc_ValueError, "%s has rows that overlap", what);
+  return t.stride(0);
+}
+int count(int64_t n, const char* what) {
+  if (n > INT32_MAX) refuse(PyExc_ValueError, "%s is too long", what);
+  return (int)n;
+}
+// `n` elements of a type side by side.
+template <typename T>
+T* flat(PyObject* o, at::ScalarType type, int64_t n, const char* what) {
+  const at::Tensor& t = here(o, what);
+  if (t.scalar_type() != type) refuse(PyExc_TypeError, "%s has the wrong element type", what);
+  if (!t.is_contiguous() || t.numel() < n) refuse(PyExc_ValueError, "%s must be contiguous and long enough", what);
+  return static_cast<T*>(t.data_ptr());
+}
+cr_mx4 mx4(PyObject* o, const char* what) {
+  cr_mx4 m{};
+  m.rows = (int)long_attr(o, s_rows);
+  m.inner = (int)long_attr(o, s_inner);
+  if (m.rows < 1 || m.inner < 1 || m.inner % 2) refuse(PyExc_ValueError, "%s has no rows, or an odd number of elements in a row", what);
+  Ref c(PyObject_GetAttr(o, s_codes)), s(PyObject_GetAttr(o, s_scales));
+  m.codes = flat<uint8_t>(c, at::kByte, (int64_t)m.rows * m.inner / 2, what);
+  m.scales = flat<uint8_t>(s, at::kByte, ((int64_t)m.rows + 127) / 128 * (((int64_t)m.inner + 127) / 128) * 512, what);
+  return m;
+}
+std::vector<cr_proj_out> projections(PyObject* outs, int64_t rows) {
+  Ref list(PySequence_Fast(outs, "outs must be a sequence"));
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(list.p);
+  std::vector<cr_proj_out> o(n);
+  int64_t col = 0;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const at::Tensor& t = here(PySequence_Fast_GET_ITEM(list.p, i), "an output");
+    if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kBFloat16) refuse(PyExc_TypeError, "%s must be float32 or bfloat16", "an output");
+    const int64_t ld = pitch(t, "an output");
+    if (t.size(0) != rows) refuse(PyExc_ValueError, "%s has another number of rows than the product", "an output");
+    o[i] = cr_proj_out{t.data_ptr(), count(col, "the outputs"), count(t.size(1), "an output"), count(ld, "an output"), t.scalar_type() == at::kFloat ? 1 : 0};
+    col += t.size(1);
+  }
+  return o;
+}
+
+PyObject* mx4_quant(PyObject*, PyObject* args) {     // (x, to)
+  return guarded([&]() -> PyObject* {
+    PyObject *x, *to;
+    if (!PyArg_ParseTuple(args, "OO", &x, &to)) throw Error();
+    const at::Tensor& xt = here(x, "x");
+    const cr_row_dtype type = row_type(xt, "x");
+    const int64_t ld = pitch(xt, "x");
+    const cr_mx4 m = mx4(to, "the 4-bit matrix");
+    if (xt.size(0) != m.rows || xt.size(1) != m.inner) refuse(PyExc_ValueError, "%s has another shape than the 4-bit matrix", "x");
+    const void* const xp = xt.data_ptr();
+    void* const st = stream();
+    check(unlocked([&] { return present(cr_mx4_quant)(xp, type, ld, &m, st); }));
+    Py_INCREF(to);
+    return to;
+  });
+}
+
+PyObject* mx4_dequant(PyObject*, PyObject* args) {   // (m, out)
+  return guarded([&]() -> PyObject* {
+    PyObject *from, *out;
+    if (!PyArg_ParseTuple(args, "OO", &from, &out)) throw Error();
+    const cr_mx4 m = mx4(from, "the 4-bit matrix");
+    const at::Tensor& t = here(out, "out");
+    const cr_row_dtype type = row_type(t, "out");
+    const int64_t ld = pitch(t, "out");
+    if (t.size(0) != m.rows || t.size(1) != m.inner) refuse(PyExc_ValueError, "%s has another shape than the 4-bit matrix", "out");
+    void *const p = t.data_ptr(), *const st = stream();
+    check(unlocked([&] { return present(cr_mx4_dequant)(&m, p, type, ld, st); }));
+    Py_INCREF(out);
+    return out;
+  });
+}
+
+PyObject* mx4_gemm(PyObject*, PyObject* args) {      // (x, w, outs)
+  return guarded([&]() -> PyObject* {
+    PyObject *x, *w, *outs;
+    if (!PyArg_ParseTuple(args, "OOO", &x, &w, &outs)) throw Error();
+    const cr_mx4 xm = mx4(x, "x"), wm = mx4(w, "w");
+    const std::vector<cr_proj_out> o = projections(outs, xm.rows);
+    void* const st = stream();
+    check(unlocked([&] { return present(cr_mx4_gemm)(&xm, &wm, o.data(), (int)o.size(), st); }));
+    Py_INCREF(outs);
+    return outs;
+  });
+}
+
+PyObject* mx4_rows(PyObject*, PyObject* args) {      // (x, w, outs)
+  return guarded([&]() -> PyObject* {
+    PyObject *x, *w, *outs;
+    if (!PyArg_ParseTuple(args, "OOO", &x, &w, &outs)) throw Error();
+    const at::Tensor& xt = here(x, "x");
+    const cr_row_dtype type = row_type(xt, "x");
+    const int64_t ld = pitch(xt, "x");
+    const cr_mx4 wm = mx4(w, "w");
+    if (xt.size(1) != wm.inner) refuse(PyExc_ValueError, "%s has another number of elements in a row than w", "x");
+    const std::vector<cr_proj_out> o = projections(outs, xt.size(0));
+    const int R = count(xt.size(0), "x");
+    const void* const xp = xt.data_ptr();
+    void* const st = stream();
+    check(unlocked([&] { return present(cr_mx4_rows)(xp, type, ld, R, &wm, o.data(), (int)o.size(), st); }));
+    Py_INCREF(outs);
+    return outs;
+  });
+}
+
+float float_or(PyObject* dict, PyObject* name, float otherwise) {
+  PyObject* o = PyDict_GetItemWithError(dict, name);
+  if (!o) { if (PyErr_Occurred()) throw Error(); return otherwise; }
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw Error();
+  return (float)v;
+}
+PyObject* item_or_none(PyObject* dict, PyObject* name) {
+  PyObject* o = PyDict_GetItemWithError(dict, name);
+  if (!o && PyErr_Occurred()) throw Error();
+  return o && o != Py_None ? o : nullptr;
+}
+PyObject* logits_choose(PyObject*, PyObject* args) { // (spans, outs or None) -> choices
+  return guarded([&]() -> PyObject* {
+    PyObject *spans, *given;
+    if (!PyArg_ParseTuple(args, "OO", &spans, &given)) throw Error();
+    Ref list(PySequence_Fast(spans, "spans must be a sequence"));
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(list.p);
+    std::vector<cr_logits_args> a(n);
+    Ref outs(PyList_New(n));
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject* sp = PySequence_Fast_GET_ITEM(list.p, i);
+      const at::Tensor& l = here(item(sp, s_logits), "logits");
+      a[i] = cr_logits_args{};
+      a[i].dtype = row_type(l, "logits");
+      a[i].ld = pitch(l, "logits");
+      a[i].logits = l.data_ptr();
+      const int R = a[i].R = count(l.size(0), "logits"), V = a[i].V = count(l.size(1), "logits");
+      if (PyObject* o = item_or_none(sp, s_out)) {
+        const at::Tensor& t = here(o, "out");
+        if (t.scalar_type() != at::kFloat) refuse(PyExc_TypeError, "%s must be float32", "out");
+        a[i].out_ld = pitch(t, "out");
+        if (t.size(0) != R || t.size(1) != V) refuse(PyExc_ValueError, "%s has another shape than the logits", "out");
+        a[i].out = static_cast<float*>(t.data_ptr());
+      }
+      if (PyObject* o = item_or_none(sp, s_counts)) a[i].counts = flat<int>(o, at::kInt, V, "counts");
+      if (PyObject* o = item_or_none(sp, s_drafts)) a[i].drafts = flat<int>(o, at::kInt, R - 1, "drafts");
+      if (PyObject* o = item_or_none(sp, s_bias)) a[i].bias = flat<float>(o, at::kFloat, V, "bias");
+      if (PyObject* o = item_or_none(sp, s_mask)) {
+        const at::Tensor& t = here(o, "mask");
+        const int64_t words = ((int64_t)V + 31) / 32;
+        if (t.scalar_type() != at::kInt) refuse(PyExc_TypeError, "%s must be int32 words", "mask");
+        if (t.dim() == 1 ? t.size(0) < words || (words > 1 && t.stride(0) != 1) : t.dim() != 2 || t.size(0) != R || t.size(1) < words)
+          refuse(PyExc_ValueError, "%s must hold a row of words, or one for each row of the logits", "mask");
+        a[i].mask = static_cast<const uint32_t*>(t.data_ptr());
+        a[i].mask_ld = t.dim() == 1 ? 0 : pitch(t, "mask");
+      }
+      a[i].repetition = float_or(sp, s_repetition, 1.f);
+      a[i].frequency = float_or(sp, s_frequency, 0.f);
+      a[i].presence = float_or(sp, s_presence, 0.f);
+      PyObject* o;
+      if (given != Py_None) {
+        o = PySequence_GetItem(given, i);
+        if (!o) throw Error();
+      } else {
+        o = wrap(at::empty({R}, at::TensorOptions().dtype(at::kInt).device(l.device())));
+      }
+      PyList_SET_ITEM(outs.p, i, o);
+      a[i].choice = flat<int>(o, at::kInt, R, "a choice");
+    }
+    void* const st = stream();
+    check(unlocked([&] { return present(cr_logits_choose)(a.data(), (int)n, st); }));
+    Py_INCREF(outs.p);
+    return outs.p;
+  });
+}
+
+PyObject* token_count(PyObject*, PyObject* args) {   // (counts, tokens, delta)
+  return guarded([&]() -> PyObject* {
+    PyObject *counts, *tokens;
+    int delta;
+    if (!PyArg_ParseTuple(args, "OOi", &counts, &tokens, &delta)) throw Error();
+    int* const c = flat<int>(counts, at::kInt, 1, "counts");
+    const int* const t = flat<int>(tokens, at::kInt, 0, "tokens");
+    const int V = count(tensor(counts).numel(), "counts"), n = count(tensor(tokens).numel(), "tokens");
+    void* const st = stream();
+    check(unlocked([&] { return present(cr_token_count)(t, n, delta, c, V, st); }));
+    Py_INCREF(counts);
+    return counts;
+  });
+}
+
 PyObject* current_stream(PyObject*, PyObject*) {
   return guarded([] { return PyLong_FromVoidPtr(stream()); });
 }
@@ -309,7 +535,10 @@ PyObject* current_stream(PyObject*, PyObject*) {
 PyMethodDef methods[] = {{"current_stream", current_stream, METH_NOARGS, nullptr},
                          {"gdn_step", gdn_step, METH_VARARGS, nullptr},       {"qsa_step", qsa_step, METH_VARARGS, nullptr},
                          {"gdn_prefill", gdn_prefill, METH_VARARGS, nullptr}, {"qsa_prefill", qsa_prefill, METH_VARARGS, nullptr},
-                         {"proj_gemm", proj_gemm, METH_VARARGS, nullptr},     {nullptr, nullptr, 0, nullptr}};
+                         {"proj_gemm", proj_gemm, METH_VARARGS, nullptr},     {"mx4_quant", mx4_quant, METH_VARARGS, nullptr},
+                         {"mx4_dequant", mx4_dequant, METH_VARARGS, nullptr}, {"mx4_gemm", mx4_gemm, METH_VARARGS, nullptr},
+                         {"mx4_rows", mx4_rows, METH_VARARGS, nullptr},       {"logits_choose", logits_choose, METH_VARARGS, nullptr},
+                         {"token_count", token_count, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

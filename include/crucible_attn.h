@@ -314,7 +314,7 @@ int cr_version(void);
  * outputs of that launch are undefined.  cr_device_status() synchronises the current device and returns the word
  * (0 = no wait has given up since the library was loaded or the word was cleared): bit 0 = tcgen05 GDN scan,
  * bit 1 = tcgen05 QSA scoring, bit 2 = tcgen05 QSA prefill attention, bit 3 = cr_debug_wait_timeout,
- * bit 4 = cr_proj_gemm.
+ * bit 4 = cr_proj_gemm, bit 5 = cr_mx4_gemm and cr_mx4_rows.
  * cr_device_check() is the same read as a status code: CR_OK or CR_ERR_TIMEOUT (cr_last_error() names the kernel).
  * cr_device_status_clear() zeroes the word.  All three synchronise: call them outside stream capture, e.g. once per
  * forward pass.  No counterpart in the reference, whose waits spin without bound
@@ -353,6 +353,78 @@ typedef struct {
  * wait that gave up. */
 cr_status cr_proj_gemm(const void* x, const void* w, int R, int K, int N, const cr_proj_out* outs, int n_outs,
                        void* stream);
+
+/* ---- 4-bit projections -------------------------------------------------------------------------------------------
+ * Matrices of microscaled 4-bit floats (MXFP4 of the OCP Microscaling Formats specification, version 1.0): blocks of 32
+ * elements of a row share a power of two.  An element is e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), a scale e8m0
+ * (byte b stands for 2^(b - 127), 255 for NaN: the whole block is NaN).  The reference's own 4-bit weights are EXL3, which stay with
+ * the engine (engine/exl3/exl3.h:85-102); these entry points are the form that Blackwell's tensor cores multiply as it lies.
+ *
+ * codes   [rows][inner / 2] bytes, element 2 i of a row in the low nibble of byte i, element 2 i + 1 in the high one
+ * scales  tiles of 128 rows x 4 blocks (512 bytes), all tiles of a row group after one another: block b of row r is byte
+ *         (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4 of tile (r / 128) * ceil(inner / 128) + b / 4.  Bytes of the last tiles that
+ *         belong to no row or block are neither written nor matter.
+ * Both 16-byte aligned.  rows >= 1, inner a multiple of 64, both below 2^24. */
+typedef struct {
+  uint8_t* codes;
+  uint8_t* scales;
+  int rows, inner;
+} cr_mx4;
+enum { CR_MX4_BLOCK = 32 };
+size_t cr_mx4_code_bytes(int rows, int inner);    /* rows * inner / 2 */
+size_t cr_mx4_scale_bytes(int rows, int inner);   /* 512 * ceil(rows / 128) * ceil(inner / 128) */
+
+/* Element types of row buffers (the values of cr_in_dtype, and fp16). */
+typedef enum { CR_ROW_F32 = 0, CR_ROW_BF16 = 1, CR_ROW_F16 = 2 } cr_row_dtype;
+
+/* Rows x [to->rows][ld] (ld >= to->inner elements, any alignment of the type) to 4 bits, the specification's conversion: with m
+ * the largest magnitude of a block, its scale is 2^s, s = floor(log2 m) - 2 held to -127..127 (-127 where m = 0), and an
+ * element becomes the e2m1 number nearest to x 2^-s, ties to the even code, 6 at most.  A block that holds an infinity or a NaN
+ * gets scale 255 and codes 0. */
+cr_status cr_mx4_quant(const void* x, cr_row_dtype dtype, long long ld, const cr_mx4* to, void* stream);
+/* The numbers that m stands for, into rows y [m->rows][ld] (rounded to the type where they do not fit it). */
+cr_status cr_mx4_dequant(const cr_mx4* m, void* y, cr_row_dtype dtype, long long ld, void* stream);
+
+/* Y[x->rows][w->rows] = X W^T, both operands of 4 bits, fp32 accumulation, the columns scattered into up to 6 outputs as
+ * cr_proj_gemm does: the projections of a prompt's rows.  x->inner = w->inner, w->rows >= 32.  Bit 5 of the device status word
+ * reports a bounded wait that gave up. */
+cr_status cr_mx4_gemm(const cr_mx4* x, const cr_mx4* w, const cr_proj_out* outs, int n_outs, void* stream);
+
+/* The same product with the rows of X as they are, [R][ld] of the given type (ld >= w->inner, any alignment of the type): the
+ * projections of decode and verify rows, and the head, where the weights' bytes set the time.  Any R >= 1; made for a few
+ * rows, each 32 of them read the weights once.  The bits of a row do not depend on the other rows of the call nor on their
+ * number. */
+cr_status cr_mx4_rows(const void* x, cr_row_dtype dtype, long long ld, int R, const cr_mx4* w, const cr_proj_out* outs,
+                      int n_outs, void* stream);
+
+/* ---- logits to tokens ----------------------------------------------------------------------------------------------
+ * Penalties for repeated tokens, biases and a grammar mask on the logits of a span, and the greedy choice (the sampler's part of
+ * Engine::Mtp / MtpSpans and of verification, engine/engine.hip:444-525; the constraint grammar of engine/runtime).  For
+ * row r and token v, in fp32 and in this order, with n = counts[v] + how many of drafts[0..r-1] are v:
+ *   l = logits[r][v]
+ *   n > 0:  l = l > 0 ? l / repetition : l * repetition
+ *           l = (l - n * frequency) - presence
+ *   l = l + bias[v];  not allowed: l = -infinity, whatever it was
+ * out[r][v] = l.  choice[r] = the lowest index among the largest allowed l (a NaN is larger than everything), -1 where the mask
+ * allows no token. */
+typedef struct {
+  const void* logits;        /* [R][ld] of `dtype`, ld >= V */
+  float* out;                /* [R][out_ld], or NULL; may be the logits themselves (fp32, the same pitch) */
+  int* choice;               /* [R], or NULL */
+  const int* counts;         /* [V] occurrences of every token so far (cr_token_count keeps them), or NULL */
+  const int* drafts;         /* [R - 1] tokens of the span's rows 1.., which later rows count too, or NULL */
+  const float* bias;         /* [V], or NULL */
+  const uint32_t* mask;      /* [R][mask_ld] words: bit v % 32 of word v / 32 set = token v is allowed; or NULL */
+  long long ld, out_ld, mask_ld;   /* mask_ld >= ceil(V / 32), or 0: one row of words for all rows */
+  int R, V;
+  cr_row_dtype dtype;
+  float repetition, frequency, presence;   /* 1, 0, 0: none.  repetition > 0; all finite */
+} cr_logits_args;
+cr_status cr_logits_choose(const cr_logits_args* spans, int n_spans, void* stream);
+
+/* counts[t] += delta for each of the n tokens (device memory; a token outside 0..V-1 is passed over): the prompt and the accepted
+ * tokens with 1, a truncated tail with -1. */
+cr_status cr_token_count(const int* tokens, int n, int delta, int* counts, int V, void* stream);
 
 /* ---- state snapshot / restore --------------------------------------------------------------------------------------
  * A span of device memory in a snapshot list.  The lists themselves (which buffers, in which order) are the host's:
