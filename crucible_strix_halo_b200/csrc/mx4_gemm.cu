@@ -1,58 +1,522 @@
-// Products with 4-bit weights: Y[R][N] = X[R][K] W[N][K]^T, W microscaled 4-bit floats, X the same (cr_mx4_gemm) or rows as they
-// are (cr_mx4_rows).
+// Product of two matrices of microscaled 4-bit floats for sm_100a: Y[R][N] = X[R][K] W[N][K]^T, fp32 accumulation, the columns
+// scattered into the outputs as cr_proj_gemm does.  tcgen05.mma.kind::mxf4 multiplies 64 elements of K per step, each block of 32 by
+// its operands' two powers of two, on the codes as they lie (packed, K-major, 128-byte-swizzled tiles of 256 elements).  The scales
+// of 128 rows x 4 blocks are one 512-byte tile of the matrix, which tcgen05.cp.32x128b.warpx4 spreads over the lanes of tensor memory as
+// the unit reads it: row r in lane r % 32 and column r / 32, its four blocks in the bytes of that word.
 //
-// mx4_simple_kernel: 64 x 64 tiles, both operands as fp32 numbers in shared memory, 4 x 4 products a thread.  A row's sums run over
-// K in order, whatever the tile.
+// A step moves the bytes of a bf16 step of 16 (4 bits against 16, four times as many), in the same cycles, so the cuts are those of
+// cr_proj_gemm with K / 4 in the place of K.
+//
+// mx4_gemm_pair_kernel (many rows): CTA pairs on 256 x 256 tiles.  Two accumulators of 256 columns would fill tensor memory and
+// leave the scales no room: they share 64 columns, which the epilogue reads first and hands over before it stores.
+// mx4_gemm_split_kernel<TN> (few rows): 128 x TN tiles, K split over a cluster of up to eight CTAs.
+//
+// The scale columns of tensor memory have two buffers.  tcgen05.cp is ordered before the products issued after it, but not behind
+// those issued before it: the issuer waits until the products of the stage before the last have completed.
+// Every wait is bounded; a wait that gives up raises bit 5 of the device status word.
+#include <cooperative_groups.h>
 #include "mx4.cuh"
 #include "proj.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace cr {
 
-constexpr int kMx4 = 3;                        // X in 4 bits, beside the row types
+CR_DEFINE_STATUS_WORD(mx4_gemm)
 
-__device__ __forceinline__ float mx4_value(const uint8_t* codes, const uint8_t* scales, int row, int k, int K, int groups) {
-  const uint32_t b = codes[(size_t)row * (K / 2) + k / 2] >> (4 * (k & 1));
-  const uint16_t h = (uint16_t)((b & 8) << 12 | (b & 7) << 9);
-  return __half2float(*reinterpret_cast<const __half*>(&h)) * 16384.f * e8m0(scales[mx4_scale_at(row, k / 32, groups)]);
+constexpr int kXM = 128, kXK = 256;                               // rows of a tile, K elements of a stage
+constexpr int kXTile = kXM * kXK / 2;                             // codes of 128 rows of a stage
+constexpr int kXScale = 2 * 512;                                  // their scales
+
+// Instruction descriptor for kind::mxf4: e2m1 operands (format 1), e8m0 scales, both operands K-major.
+__host__ __device__ constexpr uint32_t idesc_mx4(int M, int N) {
+  return (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 7) << 27);
+}
+// The two blocks of a step of 64 lie in the low (0) or the high (1) half of the scale words.
+__host__ __device__ constexpr uint32_t idesc_half(uint32_t idesc, int half) { return idesc | ((uint32_t)half << 5) | ((uint32_t)half << 30); }
+
+template <int GROUP>
+__device__ __forceinline__ void mx4_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+  if constexpr (GROUP == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+}
+// One 512-byte scale tile to four columns of tensor memory (of both CTAs of a pair, each from its own shared memory).
+template <int GROUP>
+__device__ __forceinline__ void scales_to_tmem(uint32_t col, uint64_t tile) {
+  if constexpr (GROUP == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(col), "l"(tile) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n" ::"r"(col), "l"(tile) : "memory");
+}
+// Descriptors of what a stage holds, as 16-byte steps behind the first stage's: the address is the low 14 bits of the low word, and
+// shared memory ends below their range, so that one 32-bit sum moves a descriptor.
+struct Desc {
+  uint32_t lo, hi;
+  __device__ __forceinline__ explicit Desc(uint64_t d) : lo((uint32_t)d), hi((uint32_t)(d >> 32)) {}
+  __device__ __forceinline__ uint64_t at(uint32_t bytes16) const { return (uint64_t)hi << 32 | (lo + bytes16); }
+};
+// One thread of a warp whose lanes all run the loop: the operands of the instructions stay in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}\n" : "=r"(p));
+  return p != 0;
 }
 
-template <int TYPE>
-__global__ void __launch_bounds__(256) mx4_simple_kernel(const __grid_constant__ ProjParams P, const void* __restrict__ x, const uint8_t* __restrict__ xs,
-                                                         long long ld, const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws) {
-  __shared__ float A[32][65], B[32][65];
-  pdl_release();
-  pdl_wait();
-  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64, t = threadIdx.x, tr = t / 16, tc = t % 16, groups = mx4_groups(P.K);
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < P.K; k0 += 32) {
-    for (int i = t; i < 64 * 32; i += 256) {
-      const int r = i / 32, k = i % 32;
-      float a = 0.f, b = 0.f;
-      if (m0 + r < P.R) {
-        const size_t at = (size_t)(m0 + r) * ld + k0 + k;
-        if constexpr (TYPE == kMx4) a = mx4_value(reinterpret_cast<const uint8_t*>(x), xs, m0 + r, k0 + k, P.K, groups);
-        else if constexpr (TYPE == CR_ROW_F32) a = reinterpret_cast<const float*>(x)[at];
-        else if constexpr (TYPE == CR_ROW_BF16) a = bf16_bits_to_float(reinterpret_cast<const uint16_t*>(x)[at]);
-        else a = __half2float(reinterpret_cast<const __half*>(x)[at]);
-      }
-      if (n0 + r < P.N) b = mx4_value(w, ws, n0 + r, k0 + k, P.K, groups);
-      A[k][r] = a;
-      B[k][r] = b;
+// The scales of one stage: tiles [k group] of X, [row group][k group] of W in shared memory; four columns of tensor memory per tile,
+// those of X first, then W's row groups side by side.
+template <int GROUP, int NG>
+__device__ __forceinline__ void issue_scales(uint32_t cols, const Desc& xs, const Desc& ws, uint32_t off, int steps) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (2 * k >= steps) break;
+    scales_to_tmem<GROUP>(cols + 4 * k, xs.at(off + 32 * k));
+#pragma unroll
+    for (int g = 0; g < NG; ++g) scales_to_tmem<GROUP>(cols + 8 + (k * NG + g) * 4, ws.at(off + (2 * g + k) * 32));
+  }
+}
+// The products of one stage.  sb0: columns from the first of W's scales to the tile's own first row.
+template <int GROUP, int NG>
+__device__ __forceinline__ void issue_products(uint32_t d, const Desc& xc, const Desc& wc, uint32_t off, uint32_t cols, int sb0, uint32_t idesc, int steps, bool first) {
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    if (ks >= steps) break;
+    mx4_mma<GROUP>(d, xc.at(off + ks * 2), wc.at(off + ks * 2), idesc_half(idesc, ks & 1), cols + 4 * (ks >> 1), cols + 8 + (ks >> 1) * NG * 4 + sb0,
+                   first && ks == 0 ? 0u : 1u);
+  }
+}
+
+// ---- epilogue: rows of a warp's 32 accumulator lanes to the outputs -----------------------------------------------------
+// A lane holds a row; stored from there, an instruction would touch 32 lines for 512 bytes.  The warp turns its rows through 4 KB of
+// shared memory (16-byte chunks exchanged by row, free of bank conflicts) and stores 128 or 64 bytes of a row at a time.
+// N16: 16-byte chunks of a row.
+template <int N16>
+__device__ __forceinline__ void store_turned(unsigned char* buf, const uint4 (&v)[N16], char* to, size_t pitch, int live) {
+  const int l = threadIdx.x & 31;
+#pragma unroll
+  for (int c = 0; c < N16; ++c) *reinterpret_cast<uint4*>(buf + l * 128 + ((c ^ (l & 7)) << 4)) = v[c];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < N16; ++i) {
+    const int r = i * (32 / N16) + l / N16, c = l % N16;
+    if (r < live) *reinterpret_cast<uint4*>(to + r * pitch + c * 16) = *reinterpret_cast<const uint4*>(buf + r * 128 + ((c ^ (r & 7)) << 4));
+  }
+  __syncwarp();
+}
+template <int N16>
+__device__ __forceinline__ void pack_bf16(uint4 (&p)[N16], const float* v) {
+#pragma unroll
+  for (int c = 0; c < N16; ++c) {
+    unsigned k[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __nv_bfloat162 b2 = __floats2bfloat162_rn(v[8 * c + 2 * j], v[8 * c + 2 * j + 1]);
+      k[j] = *reinterpret_cast<const unsigned*>(&b2);
     }
-    __syncthreads();
-#pragma unroll 8
-    for (int k = 0; k < 32; ++k)
+    p[c] = make_uint4(k[0], k[1], k[2], k[3]);
+  }
+}
+// Columns col .. col + 32 CH - 1 (CH: 1 or 2 chunks that an output does not divide) of `live` rows from row0 on.
+template <int CH>
+__device__ __forceinline__ void store_columns(const ProjParams& P, unsigned char* buf, int row0, int col, const float (&v)[32 * CH], int live) {
+  int o[CH];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(A[k][tr * 4 + i], B[k][tc * 4 + j], acc[i][j]);
-    __syncthreads();
+  for (int k = 0; k < CH; ++k) {
+    o[k] = 0;
+    while (o[k] < P.n_outs - 1 && col + 32 * k >= P.col0[o[k]] + P.cols[o[k]]) ++o[k];
+  }
+  auto place = [&](int k, int size) { return reinterpret_cast<char*>(P.ptr[o[k]]) + ((size_t)row0 * P.ld[o[k]] + (col + 32 * k - P.col0[o[k]])) * size; };
+  if (CH == 2 && o[0] == o[CH - 1] && !P.f32[o[0]] && col + 32 < P.N) {
+    uint4 p[4 * CH];
+    pack_bf16(p, v);
+    store_turned(buf, p, place(0, 2), (size_t)P.ld[o[0]] * 2, live);
+    return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (m0 + tr * 4 + i < P.R && n0 + tc * 4 < P.N) store_quad(P, m0 + tr * 4 + i, n0 + tc * 4, make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]));
+  for (int k = 0; k < CH; ++k) {
+    if (col + 32 * k >= P.N) return;
+    if (P.f32[o[k]]) {
+      store_turned(buf, reinterpret_cast<const uint4(&)[8]>(v[32 * k]), place(k, 4), (size_t)P.ld[o[k]] * 4, live);
+    } else {
+      uint4 p[4];
+      pack_bf16(p, v + 32 * k);
+      store_turned(buf, p, place(k, 2), (size_t)P.ld[o[k]] * 2, live);
+    }
+  }
 }
 
+// ---- CTA pairs on 256 x 256 tiles ------------------------------------------------------------------------------------
+constexpr int kQStages = 5, kQStageBytes = 2 * kXTile + 3 * kXScale, kQBand = 16;
+constexpr int kQThreads = 64 + 256;                                       // producer, issuer, eight epilogue warps
+constexpr int kQShared = 128, kQScaleCols = 512 - kQShared;               // columns that both accumulators use; first scale column
+static_assert(kQStages * 24 <= kQShared, "every stage has scale columns of its own");
+constexpr int kQTurn = kQStages * kQStageBytes;                            // 4 KB for each epilogue warp behind the stages
+constexpr size_t kQSmem = (size_t)kQTurn + 8 * 4096 + (2 * kQStages + 4) * 8 + 16;
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kQThreads, 1)
+mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
+                     const __grid_constant__ CUtensorMap xsmap, const __grid_constant__ CUtensorMap wsmap) {
+  extern __shared__ __align__(1024) unsigned char sm[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kQTurn + 8 * 4096);
+  uint64_t *full = bars, *empty = bars + kQStages, *accFull = bars + 2 * kQStages, *handed = bars + 2 * kQStages + 2;
+  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 2 * kQStages + 4);
+  volatile int& dead = *reinterpret_cast<volatile int*>(&tmem_slot + 1);
+  cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t rank = cluster.block_rank();                          // 0 leads
+  const int t = threadIdx.x, w = t >> 5, l = t & 31;
+  const int mt = (P.R + 255) / 256, nt = (P.N + 255) / 256, kb_n = (P.K + kXK - 1) / kXK, tiles = mt * nt;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  auto tile_at = [&](int i, int& m0, int& n0) {
+    const int per_band = mt * kQBand, band = i / per_band, in = i - band * per_band;
+    const int width = min(kQBand, nt - band * kQBand);
+    m0 = (in / width) * 256;
+    n0 = (band * kQBand + in % width) * 256;
+  };
+  if (t == 0) {
+    for (int i = 0; i < kQStages; ++i) { umma::mbar_init(&full[i], 1); umma::mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2; ++i) umma::mbar_init(&accFull[i], 1);
+    umma::mbar_init(handed, 16);                                          // eight epilogue warps in each CTA
+    umma::mbar_fence_init();
+    dead = (umma::smem_u32(sm) & 1023u) != 0;                           // the swizzled tiles need 1 KB boundaries
+    if (dead) g_mx4_gemm_status = 1;
+    prefetch_map(&xmap); prefetch_map(&wmap); prefetch_map(&xsmap); prefetch_map(&wsmap);
+  }
+  if (w == 1) umma::pair_tmem_alloc(&tmem_slot, 512);
+  umma::fence_before_sync();
+  cluster.sync();                                                       // both CTAs' barriers are ready
+  umma::fence_after_sync();
+  pdl_release();
+  pdl_wait();
+  const uint32_t tm = tmem_slot;
+  bool gave_up = dead;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (gave_up) return;
+    if (!umma::mbar_wait_timed(bar, parity, &dead)) { gave_up = true; dead = 1; g_mx4_gemm_status = 1; }
+  };
+
+  if (w == 0) {
+    // ---------------------------------------------------------------- producer (each CTA its own rows of X and of W, all of W's scales)
+    if (l == 0) {
+      int it = 0;
+      for (int i = pair; i < tiles && !gave_up; i += pairs) {
+        int m0, n0;
+        tile_at(i, m0, n0);
+        for (int kb = 0; kb < kb_n; ++kb, ++it) {
+          const int s = it % kQStages;
+          if (it >= kQStages) wait(&empty[s], ((it - kQStages) / kQStages) & 1);
+          if (gave_up) break;
+          unsigned char* st = sm + s * kQStageBytes;
+          if (rank == 0) umma::mbar_expect_tx(&full[s], 2 * kQStageBytes);
+          const uint32_t bar = umma::cluster_addr(&full[s], 0);
+          pair_load_box_2d(st, &xmap, kb * (kXK / 2), m0 + 128 * (int)rank, bar);
+          pair_load_box_2d(st + kXTile, &wmap, kb * (kXK / 2), n0 + 128 * (int)rank, bar);
+          pair_load_box_2d(st + 2 * kXTile, &xsmap, kb * 256, m0 / 128 + (int)rank, bar);
+          pair_load_box_2d(st + 2 * kXTile + kXScale, &wsmap, kb * 256, n0 / 128, bar);
+        }
+      }
+    }
+  } else if (w == 1) {
+    // ---------------------------------------------------------------- issuer
+    if (rank == 0) {
+      const bool one = elect_one();
+      const Desc xc(tma::desc_sw128(sm, 16, 1024)), wc(tma::desc_sw128(sm + kXTile, 16, 1024));
+      const Desc xs(umma::smem_desc(sm + 2 * kXTile, 0, 128)), ws(umma::smem_desc(sm + 2 * kXTile + kXScale, 0, 128));
+      int s = 0, phase = 0, local = 0;
+      for (int i = pair; i < tiles && !gave_up; i += pairs, ++local) {
+        const uint32_t acc = tm + (local & 1) * (256 - kQShared);
+        if (local >= 1) wait(handed, (local - 1) & 1);                     // the other accumulator's shared columns, and all of this one, have been read
+        for (int kb = 0; kb < kb_n; ++kb) {
+          wait(&full[s], phase);
+          if (gave_up) break;
+          umma::fence_after_sync();
+          const uint32_t off = s * (kQStageBytes / 16), cols = tm + kQScaleCols + s * 24;
+          const int steps = P.K / 64 - kb * 4;
+          if (one) {
+            issue_scales<2, 2>(cols, xs, ws, off, steps);
+            issue_products<2, 2>(acc, xc, wc, off, cols, 0, idesc_mx4(256, 256), steps, kb == 0);
+            umma::pair_commit(&empty[s]);                                         // the stage is free in both CTAs once these products have read it
+            if (kb == kb_n - 1) umma::pair_commit(&accFull[local & 1]);
+          }
+          if (++s == kQStages) { s = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue: two warps to each quarter of the lanes
+    const int q = w & 3, h = (w - 2) >> 2;
+    int local = 0;
+    for (int i = pair; i < tiles; i += pairs, ++local) {
+      int m0, n0;
+      tile_at(i, m0, n0);
+      const int odd = local & 1;
+      if (l == 0) wait(&accFull[odd], (local >> 1) & 1);
+      __syncwarp();
+      if (dead) break;
+      umma::fence_after_sync();
+      const int row0 = m0 + 128 * (int)rank + 32 * q, live = min(32, P.R - row0);
+#pragma unroll 1
+      for (int j = 0; j < 2; ++j) {
+        // 64 columns at a time; the shared ones are the last half of the even accumulator and the first half of the odd one
+        const int c = ((odd + j) & 1 ? 0 : 4) + 2 * h;
+        float v[64];
+        umma::tmem_ld64(umma::tmem_addr(tm, q, odd * (256 - kQShared) + 32 * c), v);     // warp-collective
+        if (j == 0) {
+          umma::fence_before_sync();
+          __syncwarp();
+          if (l == 0) umma::pair_arrive_relaxed(umma::cluster_addr(handed, 0));
+        }
+        if (live > 0 && n0 + 32 * c < P.N) store_columns<2>(P, sm + kQTurn + (w - 2) * 4096, row0, n0 + 32 * c, v, live);
+      }
+    }
+  }
+  umma::fence_before_sync();
+  __syncwarp();
+  cluster.sync();                                                          // neither CTA leaves while the other may still use its memory
+  if (w == 1) umma::pair_tmem_dealloc(tm, 512);
+}
+
+// ---- few rows: 128 x TN tiles, K split over a cluster ------------------------------------------------------------------
+// As in cr_proj_gemm: a stage holds the rows of X that exist (a multiple of 8), the MMA reads 128 all the same, and kVRing keeps a
+// whole tile behind the last stage's start.
+constexpr int kVRing = 212992, kVMaxStages = 16;
+template <int TN> constexpr int kVLd = TN + 4;                           // floats per row of a partial tile in shared memory
+constexpr size_t kVSmem = (size_t)kVRing + (2 * kVMaxStages + 1) * 8 + 16;
+constexpr int kVThreads = 64 + 256;
+template <int TN> constexpr int kVGroups = TN > 128 ? 2 : 1;             // row groups of W's scales
+template <int TN> constexpr int kVScaleCols = 8 + 8 * kVGroups<TN>;
+template <int TN> constexpr int kVCols = TN + 2 * kVScaleCols<TN> <= 128 ? 128 : (TN + 2 * kVScaleCols<TN> <= 256 ? 256 : 512);
+
+// grid: tiles x splits, cluster = splits (along x).
+template <int TN>
+__global__ void __launch_bounds__(kVThreads, 1)
+mx4_gemm_split_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
+                      const __grid_constant__ CUtensorMap xsmap, const __grid_constant__ CUtensorMap wsmap, int splits, int xrows, int ST) {
+  static_assert(128 * kVLd<TN> * 4 <= kVRing, "the partial tile takes the place of the stages");
+  extern __shared__ __align__(1024) unsigned char sm[];
+  constexpr int NG = kVGroups<TN>;
+  const int xbytes = xrows * (kXK / 2), stage = xbytes + TN * (kXK / 2) + (1 + NG) * kXScale;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kVRing);
+  uint64_t *full = bars, *empty = bars + kVMaxStages, *accFull = bars + 2 * kVMaxStages;
+  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 2 * kVMaxStages + 1);
+  volatile int& dead = *reinterpret_cast<volatile int*>(&tmem_slot + 1);
+  const int t = threadIdx.x, w = t >> 5, l = t & 31;
+  const int mt = (P.R + kXM - 1) / kXM, tile = blockIdx.x / splits, split = blockIdx.x % splits;
+  const int m0 = (tile % mt) * kXM, n0 = (tile / mt) * TN;                // row tiles of one W tile side by side
+  const int kb_all = (P.K + kXK - 1) / kXK, kb0 = kb_all * split / splits, kb_n = kb_all * (split + 1) / splits - kb0;
+  if (t == 0) {
+    for (int i = 0; i < ST; ++i) { umma::mbar_init(&full[i], 1); umma::mbar_init(&empty[i], 1); }
+    umma::mbar_init(accFull, 1);
+    umma::mbar_fence_init();
+    dead = (umma::smem_u32(sm) & 1023u) != 0;
+    if (dead) g_mx4_gemm_status = 1;
+    prefetch_map(&xmap); prefetch_map(&wmap); prefetch_map(&xsmap); prefetch_map(&wsmap);
+  }
+  if (w == 1) umma::tmem_alloc(&tmem_slot, kVCols<TN>);
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  pdl_release();
+  pdl_wait();
+  const uint32_t tm = tmem_slot;
+  bool gave_up = dead;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (gave_up) return;
+    if (!umma::mbar_wait_timed(bar, parity, &dead)) { gave_up = true; dead = 1; g_mx4_gemm_status = 1; }
+  };
+  if (w == 0) {
+    if (l == 0) {
+      for (int it = 0; it < kb_n; ++it) {
+        const int s = it % ST;
+        if (it >= ST) wait(&empty[s], (it / ST - 1) & 1);
+        if (gave_up) break;
+        unsigned char* st = sm + s * stage;
+        umma::mbar_expect_tx(&full[s], stage);
+        load_box_2d(st + xbytes, &wmap, (kb0 + it) * (kXK / 2), n0, &full[s]);
+        load_box_2d(st, &xmap, (kb0 + it) * (kXK / 2), m0, &full[s]);
+        load_box_2d(st + xbytes + TN * (kXK / 2), &xsmap, (kb0 + it) * 256, m0 / 128, &full[s]);
+        load_box_2d(st + xbytes + TN * (kXK / 2) + kXScale, &wsmap, (kb0 + it) * 256, n0 / 128, &full[s]);
+      }
+    }
+  } else if (w == 1) {
+    const bool one = elect_one();
+    const Desc xc(tma::desc_sw128(sm, 16, 1024)), wc(tma::desc_sw128(sm + xbytes, 16, 1024));
+    const Desc xs(umma::smem_desc(sm + xbytes + TN * (kXK / 2), 0, 128)), ws(umma::smem_desc(sm + xbytes + TN * (kXK / 2) + kXScale, 0, 128));
+    for (int it = 0, s = 0, phase = 0; it < kb_n; ++it) {
+      if (it >= 2) wait(&empty[(it - 2) % ST], ((it - 2) / ST) & 1);       // the scale columns' last readers are done
+      wait(&full[s], phase);
+      if (gave_up) break;
+      umma::fence_after_sync();
+      const uint32_t off = s * (stage / 16), cols = tm + TN + (it & 1) * kVScaleCols<TN>;
+      const int steps = P.K / 64 - (kb0 + it) * 4;
+      if (one) {
+        issue_scales<1, NG>(cols, xs, ws, off, steps);
+        issue_products<1, NG>(tm, xc, wc, off, cols, (n0 & 127) / 32, idesc_mx4(kXM, TN), steps, it == 0);
+        umma::commit(&empty[s]);
+        if (it == kb_n - 1) umma::commit(accFull);
+      }
+      if (++s == ST) { s = 0; phase ^= 1; }
+    }
+  } else {
+    const int q = w & 3, r = 32 * q + l;
+    if (l == 0) wait(accFull, 0);
+    __syncwarp();
+    umma::fence_after_sync();
+    if (!dead) {
+#pragma unroll 1
+      for (int c = (w - 2) >> 2; c < TN / 32; c += 2) {                     // the two warps of a lane quarter take every other chunk
+        float v[32];
+        umma::tmem_ld32(umma::tmem_addr(tm, q, 32 * c), v);                 // warp-collective
+        if (splits == 1) {
+          const int row0 = m0 + 32 * q;                                     // the stages have been read: their place serves to turn the rows
+          if (row0 < P.R && n0 + 32 * c < P.N) store_columns<1>(P, sm + (w - 2) * 4096, row0, n0 + 32 * c, v, min(32, P.R - row0));
+        } else {                                                            // the stages have been read: the partial tile goes over them
+          float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(sm) + (size_t)r * kVLd<TN> + 32 * c);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) dst[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+        }
+      }
+    }
+  }
+  umma::fence_before_sync();
+  __syncthreads();
+  if (w == 1) umma::tmem_dealloc(tm, kVCols<TN>);
+  if (splits == 1) return;
+  // Every CTA of the cluster sums a slice of the rows over all partial tiles, in the order of K.
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  const int live = min(kXM, P.R - m0), r0 = live * split / splits, r1 = live * (split + 1) / splits;
+  constexpr int kQuads = TN / 4, kFlight = 3;
+  const float* part[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) part[k] = cluster.map_shared_rank(reinterpret_cast<float*>(sm), k < splits ? k : 0);
+  for (int i0 = t; i0 < (r1 - r0) * kQuads; i0 += kFlight * kVThreads) {
+    float4 x[kFlight][8];
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const int i = i0 + f * kVThreads;
+      const size_t at = (size_t)(r0 + i / kQuads) * kVLd<TN> + (i % kQuads) * 4;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < splits && i < (r1 - r0) * kQuads) x[f][k] = *reinterpret_cast<const float4*>(part[k] + at);
+    }
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const int i = i0 + f * kVThreads, c = (i % kQuads) * 4;
+      if (i >= (r1 - r0) * kQuads || n0 + c >= P.N) continue;
+      float4 sum = x[f][0];
+#pragma unroll
+      for (int k = 1; k < 8; ++k)
+        if (k < splits) { sum.x += x[f][k].x; sum.y += x[f][k].y; sum.z += x[f][k].z; sum.w += x[f][k].w; }
+      store_quad(P, m0 + r0 + i / kQuads, n0 + c, sum);
+    }
+  }
+  cluster.sync();                                                          // the partial tiles stay until everybody has read them
+}
+
+// Codes as a tensor map of bytes with boxes of box_rows x 128 bytes, 128-byte swizzle; scales as words, a row of the map for a row
+// group, boxes of two tiles by box_groups.  Past the edges the copy engine fills in zeros.
+static cr_status map_mx4(CUtensorMap* codes, CUtensorMap* scales, const cr_mx4* m, int box_rows, int box_groups) {
+  tma::EncodeFn enc;
+  if (cr_status s = tma::encoder(&enc)) return s;
+  const cuuint32_t unit[2] = {1, 1};
+  const cuuint64_t dims[2] = {(cuuint64_t)m->inner / 2, (cuuint64_t)m->rows}, pitch[1] = {(cuuint64_t)m->inner / 2};
+  const cuuint32_t box[2] = {kXK / 2, (cuuint32_t)box_rows};
+  CUresult r = enc(codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, m->codes, dims, pitch, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) {
+    const cuuint64_t groups = mx4_groups(m->inner);
+    const cuuint64_t sdims[2] = {groups * 128, ((cuuint64_t)m->rows + 127) / 128}, spitch[1] = {groups * 512};
+    const cuuint32_t sbox[2] = {256, (cuuint32_t)box_groups};
+    r = enc(scales, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, m->scales, sdims, spitch, sbox, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  }
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed with code %d", (int)r);
+    return CR_ERR_CUDA;
+  }
+  return CR_OK;
+}
+
+// How a product is cut: the rule of cr_proj_gemm with steps of 64.  A split has to fit in one wave of the clusters that the device
+// holds at once, which the runtime is asked for.
+struct Mx4Shape { int tn, splits; };                                       // tn 0: CTA pairs
+static cr_status mx4_cluster_slots(const int (**slots)[9]) {
+  static PerDeviceOnce looked_up;
+  static int table[64][9];
+  int dev = 0;
+  CR_CUDA(cudaGetDevice(&dev));
+  if (cr_status st = once_per_device(looked_up, [dev] {
+        CR_CUDA(cudaFuncSetAttribute(mx4_gemm_split_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kVSmem));
+        for (int s = 1; s <= 8; ++s) {
+          cudaLaunchConfig_t cfg = {};
+          cfg.gridDim = dim3(s); cfg.blockDim = dim3(kVThreads); cfg.dynamicSmemBytes = kVSmem;
+          cudaLaunchAttribute attr[1];
+          attr[0].id = cudaLaunchAttributeClusterDimension;
+          attr[0].val.clusterDim.x = s; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+          cfg.attrs = attr; cfg.numAttrs = 1;
+          CR_CUDA(cudaOccupancyMaxActiveClusters(&table[dev & 63][s], mx4_gemm_split_kernel<128>, &cfg));
+        }
+        return CR_OK;
+      })) return st;
+  *slots = &table[dev & 63];
+  return CR_OK;
+}
+static Mx4Shape mx4_shape(int R, int K, int N, int sms, const int (&slots)[9]) {
+  auto up = [](long long a, long long b) { return (a + b - 1) / b; };
+  const long long stages = up(K, kXK);
+  Mx4Shape best{0, 1};
+  double cost = (double)up(up(R, 256) * up(N, 256), sms / 2) * up(K, 64) * 133 + 5000;
+  const int tns[3] = {64, 128, 256};
+  const double step[3] = {96, 132, 195};
+  for (int i = 0; i < 3; ++i) {
+    const long long tiles = up(R, kXM) * up(N, tns[i]);
+    for (int s = 1; s <= 8 && s <= stages; ++s) {
+      if (s > 1 && tiles > slots[s]) break;                                 // splitting pays only while SMs would idle
+      const double c = (double)up(tiles * s, sms) * (up(stages, s) * 4 * step[i] + 3000 + tns[i] * 10 + (s > 1 ? 2500 : 0));
+      if (c < cost) { cost = c; best = Mx4Shape{tns[i], s}; }
+    }
+  }
+  return best;
+}
+
+template <int TN>
+static cr_status mx4_split_launch(const ProjParams& P, const cr_mx4* x, const cr_mx4* w, int splits, cudaStream_t stream) {
+  static PerDeviceOnce configured;
+  if (cr_status st = once_per_device(configured, [] {
+        CR_CUDA(cudaFuncSetAttribute(mx4_gemm_split_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kVSmem));
+        return CR_OK;
+      })) return st;
+  const int xrows = P.R < kXM ? (P.R + 7) / 8 * 8 : kXM;
+  CUtensorMap xmap, wmap, xsmap, wsmap;
+  if (cr_status st = map_mx4(&xmap, &xsmap, x, xrows, 1)) return st;
+  if (cr_status st = map_mx4(&wmap, &wsmap, w, TN, kVGroups<TN>)) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(((P.R + kXM - 1) / kXM) * ((P.N + TN - 1) / TN) * splits));
+  cfg.blockDim = dim3(kVThreads);
+  cfg.dynamicSmemBytes = kVSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int na = 0;
+  if (pdl_enabled()) { attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[na++].val.programmaticStreamSerializationAllowed = 1; }
+  if (splits > 1) {
+    attr[na].id = cudaLaunchAttributeClusterDimension;
+    attr[na].val.clusterDim.x = splits; attr[na].val.clusterDim.y = 1; attr[na++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = attr; cfg.numAttrs = na;
+  const int stage = (xrows + TN) * (kXK / 2) + (1 + kVGroups<TN>) * kXScale, fit = (kVRing - (stage < kXTile ? kXTile - stage : 0)) / stage;
+  CR_CUDA(cudaLaunchKernelEx(&cfg, mx4_gemm_split_kernel<TN>, P, xmap, wmap, xsmap, wsmap, splits, xrows, fit < kVMaxStages ? fit : kVMaxStages));
+  CR_LAUNCH_CHECK("mx4_gemm_split_kernel");
+  return CR_OK;
+}
 }  // namespace cr
 
 extern "C" cr_status cr_mx4_gemm(const cr_mx4* x, const cr_mx4* w, const cr_proj_out* outs, int n_outs, void* stream_) {
@@ -62,27 +526,25 @@ extern "C" cr_status cr_mx4_gemm(const cr_mx4* x, const cr_mx4* w, const cr_proj
   CR_REQUIRE(x->inner == w->inner, "cr_mx4_gemm: X has %d elements a row, W %d", x->inner, w->inner);
   ProjParams P;
   if (cr_status s = list_outs(P, "cr_mx4_gemm", x->rows, w->inner, w->rows, outs, n_outs)) return s;
+  const int(*slots)[9];
+  if (cr_status st = mx4_cluster_slots(&slots)) return st;
+  const Mx4Shape shape = mx4_shape(P.R, P.K, P.N, sm_count(), *slots);
   cudaStream_t stream = (cudaStream_t)stream_;
   use_stream(stream);
-  CR_CUDA(launch_pdl(mx4_simple_kernel<kMx4>, dim3((P.N + 63) / 64, (P.R + 63) / 64), dim3(256), 0, stream, P, x->codes, x->scales, (long long)P.K, w->codes,
-                     w->scales));
-  CR_LAUNCH_CHECK("mx4_simple_kernel");
+  if (shape.tn == 64) return mx4_split_launch<64>(P, x, w, shape.splits, stream);
+  if (shape.tn == 128) return mx4_split_launch<128>(P, x, w, shape.splits, stream);
+  if (shape.tn == 256) return mx4_split_launch<256>(P, x, w, shape.splits, stream);
+  static PerDeviceOnce configured;
+  if (cr_status st = once_per_device(configured, [] {
+        CR_CUDA(cudaFuncSetAttribute(mx4_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kQSmem));
+        return CR_OK;
+      })) return st;
+  CUtensorMap xmap, wmap, xsmap, wsmap;
+  if (cr_status st = map_mx4(&xmap, &xsmap, x, 128, 1)) return st;
+  if (cr_status st = map_mx4(&wmap, &wsmap, w, 128, 2)) return st;
+  const long long tiles = (long long)((P.R + 255) / 256) * ((P.N + 255) / 256);
+  const int pairs = sm_count() / 2;
+  CR_CUDA(launch_pdl(mx4_gemm_pair_kernel, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), dim3(kQThreads), kQSmem, stream, P, xmap, wmap, xsmap, wsmap));
+  CR_LAUNCH_CHECK("mx4_gemm_pair_kernel");
   return CR_OK;
-}
-
-extern "C" cr_status cr_mx4_rows(const void* x, cr_row_dtype dtype, long long ld, int R, const cr_mx4* w, const cr_proj_out* outs, int n_outs, void* stream_) {
-  using namespace cr;
-  if (cr_status s = check_mx4(w, "cr_mx4_rows", "W")) return s;
-  CR_REQUIRE(R >= 1 && R < (1 << 24), "cr_mx4_rows: R=%d rows", R);
-  if (cr_status s = check_rows(x, dtype, ld, w->inner, "cr_mx4_rows")) return s;
-  ProjParams P;
-  if (cr_status s = list_outs(P, "cr_mx4_rows", R, w->inner, w->rows, outs, n_outs)) return s;
-  cudaStream_t stream = (cudaStream_t)stream_;
-  use_stream(stream);
-  return by_dtype(dtype, [&](auto type) -> cr_status {
-    CR_CUDA(launch_pdl(mx4_simple_kernel<decltype(type)::value>, dim3((P.N + 63) / 64, (P.R + 63) / 64), dim3(256), 0, stream, P, x, (const uint8_t*)nullptr, ld,
-                       w->codes, w->scales));
-    CR_LAUNCH_CHECK("mx4_simple_kernel");
-    return CR_OK;
-  });
 }

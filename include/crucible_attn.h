@@ -314,7 +314,7 @@ int cr_version(void);
  * outputs of that launch are undefined.  cr_device_status() synchronises the current device and returns the word
  * (0 = no wait has given up since the library was loaded or the word was cleared): bit 0 = tcgen05 GDN scan,
  * bit 1 = tcgen05 QSA scoring, bit 2 = tcgen05 QSA prefill attention, bit 3 = cr_debug_wait_timeout,
- * bit 4 = cr_proj_gemm, bit 5 = cr_mx4_gemm and cr_mx4_rows.
+ * bit 4 = cr_proj_gemm, bit 5 = cr_mx4_gemm.
  * cr_device_check() is the same read as a status code: CR_OK or CR_ERR_TIMEOUT (cr_last_error() names the kernel).
  * cr_device_status_clear() zeroes the word.  All three synchronise: call them outside stream capture, e.g. once per
  * forward pass.  No counterpart in the reference, whose waits spin without bound
