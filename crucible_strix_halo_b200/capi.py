@@ -133,7 +133,8 @@ _protos = {
     "cr_mx4_quant": (C.c_int, [P, C.c_int, C.c_longlong, C.POINTER(Mx4), P]),
     "cr_mx4_dequant": (C.c_int, [C.POINTER(Mx4), P, C.c_int, C.c_longlong, P]),
     "cr_mx4_gemm": (C.c_int, [C.POINTER(Mx4), C.POINTER(Mx4), C.POINTER(ProjOut), C.c_int, P]),
-    "cr_mx4_rows": (C.c_int, [P, C.c_int, C.c_longlong, C.c_int, C.POINTER(Mx4), C.POINTER(ProjOut), C.c_int, P]),
+    "cr_mx4_rows_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "cr_mx4_rows": (C.c_int, [P, C.c_int, C.c_longlong, C.c_int, C.POINTER(Mx4), P, C.c_size_t, C.POINTER(ProjOut), C.c_int, P]),
     "cr_logits_choose": (C.c_int, [C.POINTER(LogitsArgs), C.c_int, P]),
     "cr_token_count": (C.c_int, [P, C.c_int, C.c_int, P, C.c_int, P]),
     "cr_spans_bytes": (C.c_size_t, [C.POINTER(Span), C.c_int]),

@@ -104,15 +104,16 @@ extern "C" cr_status cr_set_options(const cr_options* in) {
 
 extern "C" int cr_device_status(void) {
   return cr::gdn_scan_status_read() | (cr::qsa_score_status_read() << 1) | (cr::qsa_flash_status_read() << 2) |
-         (cr::debug_wait_status_read() << 3) | (cr::proj_gemm_status_read() << 4) | (cr::mx4_gemm_status_read() << 5);
+         (cr::debug_wait_status_read() << 3) | (cr::proj_gemm_status_read() << 4) | (cr::mx4_gemm_status_read() << 5) | (cr::mx4_rows_status_read() << 6);
 }
 
 extern "C" cr_status cr_device_check(void) {
   const int st = cr_device_status();
   if (st == 0) return CR_OK;
-  cr::set_error("a bounded device-side wait gave up (status word 0x%x:%s%s%s%s%s%s); the outputs of that launch are undefined",
+  cr::set_error("a bounded device-side wait gave up (status word 0x%x:%s%s%s%s%s%s%s); the outputs of that launch are undefined",
                 st, st & 1 ? " gdn_chunk_scan_tc_kernel" : "", st & 2 ? " qsa_score_tc_kernel" : "", st & 4 ? " qsa_flash_tc_kernel" : "",
-                st & 8 ? " debug_wait_kernel" : "", st & 16 ? " proj_gemm kernels" : "", st & 32 ? " mx4_gemm kernels" : "");
+                st & 8 ? " debug_wait_kernel" : "", st & 16 ? " proj_gemm kernels" : "", st & 32 ? " mx4_gemm kernels" : "",
+                st & 64 ? " mx4_rows_kernel" : "");
   return CR_ERR_TIMEOUT;
 }
 
@@ -123,6 +124,7 @@ extern "C" cr_status cr_device_status_clear(void) {
   cr::debug_wait_status_clear();
   cr::proj_gemm_status_clear();
   cr::mx4_gemm_status_clear();
+  cr::mx4_rows_status_clear();
   CR_CUDA(cudaGetLastError());
   return CR_OK;
 }

@@ -15,6 +15,20 @@ __device__ __forceinline__ float e8m0(uint32_t b) {
   return __uint_as_float(b == 0 ? 0x00400000u : (b == 255 ? 0x7fc00000u : b << 23));
 }
 
+// Eight numbers times `by` as e2m1 codes: nearest, ties to even, 6 at most.
+__device__ __forceinline__ uint32_t pack_e2m1(const float (&v)[8], float by) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r)
+      : "f"(v[0] * by), "f"(v[1] * by), "f"(v[2] * by), "f"(v[3] * by), "f"(v[4] * by), "f"(v[5] * by), "f"(v[6] * by), "f"(v[7] * by));
+  return r;
+}
+
 // Eight consecutive elements of a row buffer as floats.  `wide`: the address is a multiple of 16 bytes.
 template <int TYPE>
 __device__ __forceinline__ void load_row8(const void* p, size_t i, bool wide, float (&v)[8]) {
@@ -64,6 +78,8 @@ inline cr_status check_rows(const void* x, int dtype, long long ld, int inner, c
   CR_REQUIRE(ld >= inner, "%s: row pitch %lld below the %d elements of a row", who, ld, inner);
   return CR_OK;
 }
+// Whether eight elements from a multiple of eight on can be read or written 16 bytes at a time.
+inline bool wide_rows(const void* p, int dtype, long long ld) { return ((uintptr_t)p & 15) == 0 && ld * (dtype == CR_ROW_F32 ? 4 : 2) % 16 == 0; }
 // Calls f with an integral constant of the element type.
 template <typename F>
 inline cr_status by_dtype(int dtype, F&& f) {

@@ -7,19 +7,6 @@
 
 namespace cr {
 
-__device__ __forceinline__ uint32_t pack_e2m1(const float (&v)[8], float by) {
-  uint32_t r;
-  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
-      "mov.b32 %0, {a, b, c, d};\n\t}"
-      : "=r"(r)
-      : "f"(v[0] * by), "f"(v[1] * by), "f"(v[2] * by), "f"(v[3] * by), "f"(v[4] * by), "f"(v[5] * by), "f"(v[6] * by), "f"(v[7] * by));
-  return r;
-}
-
 template <int TYPE>
 __global__ void __launch_bounds__(256) mx4_quant_kernel(const void* __restrict__ x, long long ld, bool wide, uint8_t* __restrict__ codes,
                                                         uint8_t* __restrict__ scales, int rows, int inner) {
@@ -96,7 +83,6 @@ static dim3 unit_grid(int rows, int inner) {
   const long long blocks = ((long long)rows * (inner / 8) + 255) / 256, most = (long long)sm_count() * 8;
   return dim3((unsigned)(blocks < most ? blocks : most));
 }
-static bool wide_rows(const void* p, int dtype, long long ld) { return ((uintptr_t)p & 15) == 0 && ld * (dtype == CR_ROW_F32 ? 4 : 2) % 16 == 0; }
 
 }  // namespace cr
 

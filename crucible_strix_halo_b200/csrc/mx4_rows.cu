@@ -1,68 +1,319 @@
-// Products with 4-bit weights: Y[R][N] = X[R][K] W[N][K]^T, W microscaled 4-bit floats, X rows as they are.
+// Products of a few rows with 4-bit weights for sm_100a: Y[R][N] = X[R][K] W[N][K]^T, W microscaled 4-bit floats, X fp32, bf16 or
+// fp16 rows as they are: the projections of decode and verify rows, and the head.  W's bytes set the time.
 //
-// mx4_simple_kernel: 64 x 64 tiles, both operands as fp32 numbers in shared memory, 4 x 4 products a thread.  A row's sums run over
-// K in order, whatever the tile.
-#include "mx4.cuh"
-#include "proj.cuh"
+// Turning the weights into numbers that X could be multiplied with costs more instructions than an SM has while it receives them:
+// with mma.sync on unpacked weights 131,072 x 2,048 took 72 us for one row and 114 for nine, 3 to 5 times the weights' own 22.  Here
+// X is turned into 4-bit numbers instead, without loss, and the tensor cores multiply the weights as they lie:
+//   x = sum over j = 0.. of d_j 2^(E - 2 - 3 j),  d_j = the whole number in -4..4 nearest to what the digits before it left,
+// with 2^E above the largest of x's block of 32.  A digit is an e2m1 number and its weight an e8m0 scale, so that the digits of a row
+// are rows of a 4-bit matrix.  Ten of them for bf16 and fp16 rows, twelve for fp32 rows: an element is off by at most 2^(E - 30) or
+// 2^(E - 36), and exact where it has no bits below twice that, so that a channel a thousand times the others' size takes
+// nothing from them.  The sums of an output's digits, each in fp32, are added from the smallest up.  The order of all sums depends on N
+// and K alone: a row has the same bits in every call.
+//
+// mx4_digits_kernel writes the digits into the workspace, a block of 256 rows for each pass over W.  mx4_rows_kernel multiplies: 128 rows of W are the M side, up to
+// 256 digit rows the N side; persistent over W, or one tile per cluster of CTAs that share K where there are few tiles.  The first
+// stages of W are asked for while the digits are still being made.
+#include <cooperative_groups.h>
+#include "mx4_mma.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace cr {
 
-__device__ __forceinline__ float mx4_value(const uint8_t* codes, const uint8_t* scales, int row, int k, int K, int groups) {
-  const uint32_t b = codes[(size_t)row * (K / 2) + k / 2] >> (4 * (k & 1));
-  const uint16_t h = (uint16_t)((b & 8) << 12 | (b & 7) << 9);
-  return __half2float(*reinterpret_cast<const __half*>(&h)) * 16384.f * e8m0(scales[mx4_scale_at(row, k / 32, groups)]);
+CR_DEFINE_STATUS_WORD(mx4_rows)
+
+constexpr int kDigitsMost = 12, kPassRows = 256;                 // digit rows of a pass over W
+__host__ __device__ constexpr int digits_of(int dtype) { return dtype == CR_ROW_F32 ? 12 : 10; }
+constexpr int kNThreads = 192;                                   // producer, issuer, four epilogue warps
+constexpr int kNMaxStages = 8;
+constexpr size_t kNRing = 212992;
+constexpr size_t kNSmem = kNRing + (2 * kNMaxStages + 4) * 8 + 16;
+
+// ---- digits ----------------------------------------------------------------------------------------------------------
+// A thread takes eight elements of a block.
+template <int TYPE>
+__global__ void __launch_bounds__(128) mx4_digits_kernel(const void* __restrict__ x, long long ld, bool wide, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                         int rows, int inner, int pass_rows) {
+  constexpr int D = digits_of(TYPE);
+  // What stands before this kernel on the stream has ended when the kernel behind it is let in: that one reads the weights at once.
+  pdl_wait();
+  pdl_release();
+  const int per_row = inner / 8, groups = mx4_groups(inner);
+  const long long u = (long long)blockIdx.x * 128 + threadIdx.x;
+  if (u >= (long long)rows * per_row) return;                      // a multiple of eight threads
+  const int row = (int)(u / per_row), i = (int)(u - (long long)row * per_row);
+  float v[8];
+  load_row8<TYPE>(x, (size_t)row * ld + (size_t)i * 8, wide, v);
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
+  const unsigned four = 0xfu << (threadIdx.x & 28);
+  top = max(top, __shfl_xor_sync(four, top, 1));
+  top = max(top, __shfl_xor_sync(four, top, 2));
+  const int field = max((int)(top >> 23), 1);                      // 2^(field - 126) is above every element; 255: not finite
+  const float up = __uint_as_float((uint32_t)(field == 255 ? 1 : 255 - field) << 23);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] *= up;                          // below 4
+  const int at = row / pass_rows * kPassRows + row % pass_rows * D;
+  uint32_t* to = reinterpret_cast<uint32_t*>(codes) + (size_t)at * per_row + i;
+#pragma unroll
+  for (int j = 0; j < D; ++j) {
+    const int scale = field - 1 - 3 * j;                           // below 0: what is left lies under 2^-127
+    float d[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      d[k] = rintf(v[k]);
+      v[k] = (v[k] - d[k]) * 8.f;
+    }
+    to[(size_t)j * per_row] = field == 255 || scale < 0 ? 0u : pack_e2m1(d, 1.f);
+    if ((threadIdx.x & 3) == 0) scales[mx4_scale_at(at + j, i >> 2, groups)] = field == 255 ? 255 : (uint8_t)max(scale, 0);
+  }
 }
 
-template <int TYPE>
-__global__ void __launch_bounds__(256) mx4_simple_kernel(const __grid_constant__ ProjParams P, const void* __restrict__ x, long long ld, const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws) {
-  __shared__ float A[32][65], B[32][65];
-  pdl_release();
-  pdl_wait();
-  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64, t = threadIdx.x, tr = t / 16, tc = t % 16, groups = mx4_groups(P.K);
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < P.K; k0 += 32) {
-    for (int i = t; i < 64 * 32; i += 256) {
-      const int r = i / 32, k = i % 32;
-      float a = 0.f, b = 0.f;
-      if (m0 + r < P.R) {
-        const size_t at = (size_t)(m0 + r) * ld + k0 + k;
-        if constexpr (TYPE == CR_ROW_F32) a = reinterpret_cast<const float*>(x)[at];
-        else if constexpr (TYPE == CR_ROW_BF16) a = bf16_bits_to_float(reinterpret_cast<const uint16_t*>(x)[at]);
-        else a = __half2float(reinterpret_cast<const __half*>(x)[at]);
-      }
-      if (n0 + r < P.N) b = mx4_value(w, ws, n0 + r, k0 + k, P.K, groups);
-      A[k][r] = a;
-      B[k][r] = b;
-    }
-    __syncthreads();
-#pragma unroll 8
-    for (int k = 0; k < 32; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(A[k][tr * 4 + i], B[k][tc * 4 + j], acc[i][j]);
-    __syncthreads();
+// ---- product ----------------------------------------------------------------------------------------------------------------
+struct RowsShape {
+  int splits, tiles, passes, pass_rows;                            // CTAs that share K; tiles of W; passes over W, rows of X in each
+  int digits, cols;                                                // digits of an element; digit rows of a pass, a multiple of 8
+  int stages, stage;                                               // the ring and its stages' bytes
+};
+
+__global__ void __launch_bounds__(kNThreads, 1)
+mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ RowsShape S, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
+                const __grid_constant__ CUtensorMap wsmap, const __grid_constant__ CUtensorMap xsmap) {
+  extern __shared__ __align__(1024) unsigned char sm[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kNRing);
+  uint64_t *full = bars, *empty = bars + kNMaxStages, *accFull = bars + 2 * kNMaxStages, *accEmpty = bars + 2 * kNMaxStages + 2;
+  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 2 * kNMaxStages + 4);
+  volatile int& dead = *reinterpret_cast<volatile int*>(&tmem_slot + 1);
+  const int t = threadIdx.x, w = t >> 5, l = t & 31;
+  const int split = blockIdx.x % S.splits, first = blockIdx.x / S.splits, step = gridDim.x / S.splits, units = S.tiles * S.passes;
+  const int kb_all = (P.K + kXK - 1) / kXK, kb0 = kb_all * split / S.splits, kb_n = kb_all * (split + 1) / S.splits - kb0;
+  const int xbytes = S.cols * (kXK / 2), ST = S.stages, two = S.cols > 128;
+  const int accs = two ? 1 : 2, acc_cols = (S.cols + 31) / 32 * 32, scale_cols = two ? 24 : 16;
+  if (t == 0) {
+    for (int i = 0; i < ST; ++i) { umma::mbar_init(&full[i], 1); umma::mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { umma::mbar_init(&accFull[i], 1); umma::mbar_init(&accEmpty[i], 4); }
+    umma::mbar_fence_init();
+    dead = (umma::smem_u32(sm) & 1023u) != 0;                        // the swizzled tiles need 1 KB boundaries
+    if (dead) g_mx4_rows_status = 1;
+    prefetch_map(&wmap); prefetch_map(&xmap); prefetch_map(&wsmap); prefetch_map(&xsmap);
   }
+  if (w == 1) umma::tmem_alloc(&tmem_slot, 512);
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  pdl_release();
+  const uint32_t tm = tmem_slot;
+  bool gave_up = dead;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (gave_up) return;
+    if (!umma::mbar_wait_timed(bar, parity, &dead)) { gave_up = true; dead = 1; g_mx4_rows_status = 1; }
+  };
+  // A unit is a tile of W and a pass; the passes of a tile follow one another.  Stage: codes of W, scales of W, codes of X, scales of X.
+  if (w == 0) {
+    if (l == 0) {
+      const int own = first < units ? (units - first + step - 1) / step : 0, all = own * kb_n;
+      auto load_w = [&](int it) {
+        unsigned char* st = sm + it % ST * S.stage;
+        uint64_t* bar = &full[it % ST];
+        const int n0 = (first + it / kb_n * step) / S.passes * 128, kb = kb0 + it % kb_n;
+        umma::mbar_expect_tx(bar, S.stage);
+        load_box_2d(st, &wmap, kb * (kXK / 2), n0, bar);
+        load_box_2d(st + kXTile, &wsmap, kb * 256, n0 / 128, bar);
+      };
+      auto load_x = [&](int it) {
+        unsigned char* st = sm + it % ST * S.stage + kXTile + kXScale;
+        uint64_t* bar = &full[it % ST];
+        const int pass = (first + it / kb_n * step) % S.passes, kb = kb0 + it % kb_n;
+        load_box_2d(st + kXScale * (1 + two), &xmap, kb * (kXK / 2), pass * kPassRows, bar);
+        load_box_2d(st, &xsmap, kb * 256, pass * (kPassRows / 128), bar);
+      };
+      const int ahead = min(ST, all);
+      for (int it = 0; it < ahead; ++it) load_w(it);
+      pdl_wait();
+      for (int it = 0; it < ahead; ++it) load_x(it);
+      for (int it = ahead; it < all; ++it) {
+        wait(&empty[it % ST], (it / ST - 1) & 1);
+        if (gave_up) break;
+        load_w(it);
+        load_x(it);
+      }
+    }
+  } else if (w == 1) {
+    const bool one = elect_one();
+    const Desc wc(tma::desc_sw128(sm, 16, 1024)), xc(tma::desc_sw128(sm + kXTile + kXScale * (2 + two), 16, 1024));
+    const Desc ws(umma::smem_desc(sm + kXTile, 0, 128)), xs(umma::smem_desc(sm + kXTile + kXScale, 0, 128));
+    const uint32_t idesc = idesc_mx4(kXM, S.cols), scales = tm + accs * acc_cols;
+    int s = 0, phase = 0, local = 0;
+    for (int u = first; u < units && !gave_up; u += step, ++local) {
+      const int a = two ? 0 : local & 1, use = two ? local : local >> 1;
+      if (use >= 1) wait(&accEmpty[a], (use - 1) & 1);
+      for (int kb = 0; kb < kb_n; ++kb) {
+        wait(&full[s], phase);
+        if (gave_up) break;
+        umma::fence_after_sync();
+        const uint32_t off = s * (S.stage / 16), cols = scales + s * scale_cols;
+        const int steps = P.K / 64 - (kb0 + kb) * 4;
+        if (one) {
+          if (two) {
+            issue_scales<1, 2>(cols, ws, xs, off, steps);
+            issue_products<1, 2>(tm + a * acc_cols, wc, xc, off, cols, 0, idesc, steps, kb == 0);
+          } else {
+            issue_scales<1, 1>(cols, ws, xs, off, steps);
+            issue_products<1, 1>(tm + a * acc_cols, wc, xc, off, cols, 0, idesc, steps, kb == 0);
+          }
+          umma::commit(&empty[s]);
+          if (kb == kb_n - 1) umma::commit(&accFull[a]);
+        }
+        if (++s == ST) { s = 0; phase ^= 1; }
+      }
+    }
+  } else {
+    const int q = w & 3;
+    int local = 0;
+    for (int u = first; u < units; u += step, ++local) {
+      const int a = two ? 0 : local & 1, use = two ? local : local >> 1;
+      const int n0 = u / S.passes * 128 + 32 * q, r0 = u % S.passes * S.pass_rows, live = min(S.pass_rows, P.R - r0);
+      if (l == 0) wait(&accFull[a], use & 1);
+      __syncwarp();
+      if (dead) break;
+      umma::fence_after_sync();
+      int o = 0;
+      while (o < P.n_outs - 1 && n0 >= P.col0[o] + P.cols[o]) ++o;     // 32 columns never straddle outputs
+#pragma unroll 1
+      for (int r = 0; r < live; ++r) {
+        float v[16];
+        umma::tmem_ld16(umma::tmem_addr(tm, q, a * acc_cols + r * S.digits), v);     // warp-collective
+        if (r + 1 == live) {
+          umma::fence_before_sync();
+          __syncwarp();
+          if (l == 0) umma::mbar_arrive_relaxed(&accEmpty[a]);
+        }
+        float y = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (m0 + tr * 4 + i < P.R && n0 + tc * 4 < P.N) store_quad(P, m0 + tr * 4 + i, n0 + tc * 4, make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]));
+        for (int j = kDigitsMost - 1; j >= 0; --j)
+          if (j < S.digits) y += v[j];
+        if (S.splits > 1) {
+          reinterpret_cast<float*>(sm)[r * 128 + 32 * q + l] = y;                     // every stage has been read
+        } else if (n0 < P.N) {
+          const size_t at = (size_t)(r0 + r) * P.ld[o] + (n0 + l - P.col0[o]);
+          if (P.f32[o]) reinterpret_cast<float*>(P.ptr[o])[at] = y;
+          else reinterpret_cast<__nv_bfloat16*>(P.ptr[o])[at] = __float2bfloat16_rn(y);
+        }
+      }
+    }
+  }
+  umma::fence_before_sync();
+  __syncthreads();
+  if (w == 1) umma::tmem_dealloc(tm, 512);
+  if (S.splits == 1) return;
+  // One unit per cluster: each CTA adds a part of the outputs over all shares of K, in their order.
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  const int n0 = first / S.passes * 128, r0 = first % S.passes * S.pass_rows, outs = min(S.pass_rows, P.R - r0) * 128;
+  for (int i = outs * split / S.splits + t; i < outs * (split + 1) / S.splits; i += kNThreads) {
+    float y = 0.f;
+    for (int k = 0; k < S.splits; ++k) y += *cluster.map_shared_rank(reinterpret_cast<float*>(sm) + i, k);
+    const int col = n0 + i % 128;
+    if (col >= P.N) continue;
+    int o = 0;
+    while (o < P.n_outs - 1 && col >= P.col0[o] + P.cols[o]) ++o;
+    const size_t at = (size_t)(r0 + i / 128) * P.ld[o] + (col - P.col0[o]);
+    if (P.f32[o]) reinterpret_cast<float*>(P.ptr[o])[at] = y;
+    else reinterpret_cast<__nv_bfloat16*>(P.ptr[o])[at] = __float2bfloat16_rn(y);
+  }
+  cluster.sync();                                                       // the parts stay until everybody has read them
+}
+
+// CTAs that share K: as many as give every SM a tile, while all clusters run at once.  R has no part in it.
+static cr_status rows_splits(int N, int K, int* splits) {
+  static PerDeviceOnce configured;
+  static int slots[64][9];
+  int dev = 0;
+  CR_CUDA(cudaGetDevice(&dev));
+  if (cr_status st = once_per_device(configured, [dev] {
+        CR_CUDA(cudaFuncSetAttribute(mx4_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kNSmem));
+        for (int s = 1; s <= 8; ++s) {
+          cudaLaunchConfig_t cfg = {};
+          cfg.gridDim = dim3(s); cfg.blockDim = dim3(kNThreads); cfg.dynamicSmemBytes = kNSmem;
+          cudaLaunchAttribute attr[1];
+          attr[0].id = cudaLaunchAttributeClusterDimension;
+          attr[0].val.clusterDim.x = s; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+          cfg.attrs = attr; cfg.numAttrs = 1;
+          CR_CUDA(cudaOccupancyMaxActiveClusters(&slots[dev & 63][s], mx4_rows_kernel, &cfg));
+        }
+        return CR_OK;
+      })) return st;
+  const int tiles = (N + 127) / 128, stages = (K + kXK - 1) / kXK;
+  *splits = 1;
+  for (int s = 2; s <= 8 && s <= stages; ++s)
+    if (tiles <= slots[dev & 63][s]) *splits = s;
+  return CR_OK;
 }
 
 }  // namespace cr
 
-extern "C" cr_status cr_mx4_rows(const void* x, cr_row_dtype dtype, long long ld, int R, const cr_mx4* w, const cr_proj_out* outs, int n_outs, void* stream_) {
+// Passes over W of R rows: as few as hold them, with as many rows in each.
+static int rows_passes(int R, int digits) {
+  const int most = cr::kPassRows / digits;
+  return (R + most - 1) / most;
+}
+extern "C" size_t cr_mx4_rows_workspace_bytes(int R, int inner) {
+  if (R < 1 || inner < 1) return 0;
+  const int rows = rows_passes(R, cr::kDigitsMost) * cr::kPassRows;
+  return cr_mx4_code_bytes(rows, inner) + cr_mx4_scale_bytes(rows, inner);
+}
+
+extern "C" cr_status cr_mx4_rows(const void* x, cr_row_dtype dtype, long long ld, int R, const cr_mx4* w, void* workspace, size_t workspace_bytes,
+                                 const cr_proj_out* outs, int n_outs, void* stream_) {
   using namespace cr;
   if (cr_status s = check_mx4(w, "cr_mx4_rows", "W")) return s;
-  CR_REQUIRE(R >= 1 && R < (1 << 24), "cr_mx4_rows: R=%d rows", R);
+  CR_REQUIRE(R >= 1 && R < (1 << 20), "cr_mx4_rows: R=%d rows", R);
   if (cr_status s = check_rows(x, dtype, ld, w->inner, "cr_mx4_rows")) return s;
+  CR_REQUIRE((long long)R * w->inner < (1ll << 35) && (long long)R * w->rows < (1ll << 40), "cr_mx4_rows: %d rows of %d x %d are too many for a call", R, w->rows, w->inner);
+  CR_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= cr_mx4_rows_workspace_bytes(R, w->inner),
+             "cr_mx4_rows: the workspace must hold %zu bytes at a 16-byte boundary", cr_mx4_rows_workspace_bytes(R, w->inner));
   ProjParams P;
   if (cr_status s = list_outs(P, "cr_mx4_rows", R, w->inner, w->rows, outs, n_outs)) return s;
+  RowsShape S{};
+  if (cr_status s = rows_splits(P.N, P.K, &S.splits)) return s;
+  S.tiles = (P.N + 127) / 128;
+  S.digits = digits_of(dtype);
+  S.passes = rows_passes(R, S.digits);
+  S.pass_rows = (R + S.passes - 1) / S.passes;
+  S.cols = (S.digits * S.pass_rows + 7) / 8 * 8;
+  cr_mx4 d{static_cast<uint8_t*>(workspace), nullptr, S.passes * kPassRows, w->inner};
+  d.scales = d.codes + cr_mx4_code_bytes(d.rows, d.inner);
+  S.stage = kXTile + S.cols * (kXK / 2) + (S.cols > 128 ? 3 : 2) * kXScale;
+  S.stages = (int)(kNRing / S.stage < kNMaxStages ? kNRing / S.stage : kNMaxStages);
+  CUtensorMap wmap, wsmap, xmap, xsmap;
+  if (cr_status s = map_mx4(&wmap, &wsmap, w, 128, 1)) return s;
+  if (cr_status s = map_mx4(&xmap, &xsmap, &d, S.cols, S.cols > 128 ? 2 : 1)) return s;
   cudaStream_t stream = (cudaStream_t)stream_;
   use_stream(stream);
-  return by_dtype(dtype, [&](auto type) -> cr_status {
-    CR_CUDA(launch_pdl(mx4_simple_kernel<decltype(type)::value>, dim3((P.N + 63) / 64, (P.R + 63) / 64), dim3(256), 0, stream, P, x, ld,
-                       w->codes, w->scales));
-    CR_LAUNCH_CHECK("mx4_simple_kernel");
-    return CR_OK;
-  });
+  if (cr_status s = by_dtype(dtype, [&](auto type) -> cr_status {
+        const long long threads = (long long)R * (w->inner / 8);
+        CR_CUDA(launch_pdl(mx4_digits_kernel<decltype(type)::value>, dim3((unsigned)((threads + 127) / 128)), dim3(128), 0, stream, x, ld, wide_rows(x, dtype, ld),
+                           d.codes, d.scales, R, w->inner, S.pass_rows));
+        CR_LAUNCH_CHECK("mx4_digits_kernel");
+        return CR_OK;
+      })) return s;
+  const long long units = (long long)S.tiles * S.passes;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(S.splits > 1 ? units * S.splits : (units < sm_count() ? units : sm_count())));
+  cfg.blockDim = dim3(kNThreads);
+  cfg.dynamicSmemBytes = kNSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int na = 0;
+  if (pdl_enabled()) { attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[na++].val.programmaticStreamSerializationAllowed = 1; }
+  if (S.splits > 1) {
+    attr[na].id = cudaLaunchAttributeClusterDimension;
+    attr[na].val.clusterDim.x = S.splits; attr[na].val.clusterDim.y = 1; attr[na++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = attr; cfg.numAttrs = na;
+  CR_CUDA(cudaLaunchKernelEx(&cfg, mx4_rows_kernel, P, S, wmap, xmap, wsmap, xsmap));
+  CR_LAUNCH_CHECK("mx4_rows_kernel");
+  return CR_OK;
 }

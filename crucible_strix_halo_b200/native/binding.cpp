@@ -15,6 +15,7 @@
 #pragma weak cr_mx4_dequant
 #pragma weak cr_mx4_gemm
 #pragma weak cr_mx4_rows
+#pragma weak cr_mx4_rows_workspace_bytes
 #pragma weak cr_logits_choose
 #pragma weak cr_token_count
 
@@ -438,9 +439,12 @@ PyObject* mx4_rows(PyObject*, PyObject* args) {      // (x, w, outs)
     if (xt.size(1) != wm.inner) refuse(PyExc_ValueError, "%s has another number of elements in a row than w", "x");
     const std::vector<cr_proj_out> o = projections(outs, xt.size(0));
     const int R = count(xt.size(0), "x");
+    const size_t bytes = present(cr_mx4_rows_workspace_bytes)(R, wm.inner);
+    const at::Tensor ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(xt.device()));   // of the current stream
+    void* const wsp = ws.data_ptr();
     const void* const xp = xt.data_ptr();
     void* const st = stream();
-    check(unlocked([&] { return present(cr_mx4_rows)(xp, type, ld, R, &wm, o.data(), (int)o.size(), st); }));
+    check(unlocked([&] { return present(cr_mx4_rows)(xp, type, ld, R, &wm, wsp, bytes, o.data(), (int)o.size(), st); }));
     Py_INCREF(outs);
     return outs;
   });

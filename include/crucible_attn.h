@@ -314,7 +314,7 @@ int cr_version(void);
  * outputs of that launch are undefined.  cr_device_status() synchronises the current device and returns the word
  * (0 = no wait has given up since the library was loaded or the word was cleared): bit 0 = tcgen05 GDN scan,
  * bit 1 = tcgen05 QSA scoring, bit 2 = tcgen05 QSA prefill attention, bit 3 = cr_debug_wait_timeout,
- * bit 4 = cr_proj_gemm, bit 5 = cr_mx4_gemm.
+ * bit 4 = cr_proj_gemm, bit 5 = cr_mx4_gemm, bit 6 = cr_mx4_rows.
  * cr_device_check() is the same read as a status code: CR_OK or CR_ERR_TIMEOUT (cr_last_error() names the kernel).
  * cr_device_status_clear() zeroes the word.  All three synchronise: call them outside stream capture, e.g. once per
  * forward pass.  No counterpart in the reference, whose waits spin without bound
@@ -391,11 +391,14 @@ cr_status cr_mx4_dequant(const cr_mx4* m, void* y, cr_row_dtype dtype, long long
 cr_status cr_mx4_gemm(const cr_mx4* x, const cr_mx4* w, const cr_proj_out* outs, int n_outs, void* stream);
 
 /* The same product with the rows of X as they are, [R][ld] of the given type (ld >= w->inner, any alignment of the type): the
- * projections of decode and verify rows, and the head, where the weights' bytes set the time.  Any R >= 1; made for a few
- * rows, each 32 of them read the weights once.  The bits of a row do not depend on the other rows of the call nor on their
- * number. */
-cr_status cr_mx4_rows(const void* x, cr_row_dtype dtype, long long ld, int R, const cr_mx4* w, const cr_proj_out* outs,
-                      int n_outs, void* stream);
+ * projections of decode and verify rows, and the head, where the weights' bytes set the time.  Any R in 1..2^20 - 1; made for a few
+ * rows, each 25 of them (21 of fp32) read the weights once.  X enters as 4-bit digits: an element is off by at most 2^-30 (fp32:
+ * 2^-36) of the power of two above the largest of its block of 32, and what lies under 2^-127 is left out.  The bits of a row do not
+ * depend on the other rows of the call nor on their number.  A row that holds an infinity or a NaN gives NaN.  `workspace`: cr_mx4_rows_workspace_bytes(R, w->inner) bytes,
+ * 16-byte aligned, of this call alone until it has run.  Bit 6 of the device status word reports a bounded wait that gave up. */
+size_t cr_mx4_rows_workspace_bytes(int R, int inner);
+cr_status cr_mx4_rows(const void* x, cr_row_dtype dtype, long long ld, int R, const cr_mx4* w, void* workspace,
+                      size_t workspace_bytes, const cr_proj_out* outs, int n_outs, void* stream);
 
 /* ---- logits to tokens ----------------------------------------------------------------------------------------------
  * Penalties for repeated tokens, biases and a grammar mask on the logits of a span, and the greedy choice (the sampler's part of

@@ -272,16 +272,13 @@ def test_blocks_that_are_nan_reach_their_own_outputs_alone(call, R):
 
 
 @pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
-def test_a_row_that_is_not_finite_leaves_the_others(value):
+def test_a_row_that_is_not_finite_is_nan_and_leaves_the_others(value):
     L = layers()
     x, w = torch.randn(9, 128, device="cuda"), random_mx4(64, 128, 2)
-    w.codes[:, 10] = 0x22                                       # elements 20 and 21 are 1
     x[4, 20] = value
     y = torch.empty(9, 64, device="cuda")
     L.mx4_rows(x, w, [y])
-    assert torch.equal(y[4].isnan(), torch.full((64,), math.isnan(value), device="cuda"))
-    if not math.isnan(value):
-        assert (y[4] == value).all()
+    assert y[4].isnan().all()
     keep = [0, 1, 2, 3, 5, 6, 7, 8]
     check_product(x[keep].double().cpu(), values64(w), [y[keep]], 128)
 

@@ -38,7 +38,7 @@ def test_matrices_that_are_refused(capi, bad):
     assert lib.cr_mx4_dequant(m, BASE, capi.ROW_F32, 1 << 24, None) == capi.ERR_INVALID
     assert lib.cr_mx4_gemm(m, ok, out, 1, None) == capi.ERR_INVALID
     assert lib.cr_mx4_gemm(ok, m, out, 1, None) == capi.ERR_INVALID
-    assert lib.cr_mx4_rows(BASE, capi.ROW_F32, 1 << 24, 1, m, out, 1, None) == capi.ERR_INVALID
+    assert lib.cr_mx4_rows(BASE, capi.ROW_F32, 1 << 24, 1, m, BASE, 1 << 30, out, 1, None) == capi.ERR_INVALID
     assert lib.cr_mx4_quant(BASE, capi.ROW_F32, 64, None, None) == capi.ERR_INVALID
 
 
@@ -47,7 +47,7 @@ def test_matrices_that_are_refused(capi, bad):
 def test_rows_that_are_refused(capi, x, dtype, ld, R):
     lib, m = capi.lib, _mx4(capi)
     out = (capi.ProjOut * 1)(capi.ProjOut(BASE, 0, 32, 32, 1))
-    assert lib.cr_mx4_rows(x, dtype, ld, R, m, out, 1, None) == capi.ERR_INVALID
+    assert lib.cr_mx4_rows(x, dtype, ld, R, m, BASE, 1 << 30, out, 1, None) == capi.ERR_INVALID
     if R == 1:
         assert lib.cr_mx4_quant(x, dtype, ld, m, None) == capi.ERR_INVALID
         assert lib.cr_mx4_dequant(m, x, dtype, ld, None) == capi.ERR_INVALID
@@ -59,7 +59,16 @@ def test_outputs_that_are_refused(capi, outs):
     lib, m = capi.lib, _mx4(capi)
     o = (capi.ProjOut * max(1, len(outs)))(*[capi.ProjOut(*x) for x in outs])
     assert lib.cr_mx4_gemm(m, m, o, len(outs), None) == capi.ERR_INVALID
-    assert lib.cr_mx4_rows(BASE, 0, 64, 1, m, o, len(outs), None) == capi.ERR_INVALID
+    assert lib.cr_mx4_rows(BASE, 0, 64, 1, m, BASE, 1 << 30, o, len(outs), None) == capi.ERR_INVALID
+
+
+@pytest.mark.parametrize("workspace,short", [(None, 0), (BASE + 8, 0), (BASE, 1)])
+def test_workspaces_that_are_refused(capi, workspace, short):
+    lib = capi.lib
+    out = (capi.ProjOut * 1)(capi.ProjOut(BASE, 0, 32, 32, 1))
+    need = lib.cr_mx4_rows_workspace_bytes(3, 192)
+    assert need == 256 * 96 + 4 * 512 and lib.cr_mx4_rows_workspace_bytes(0, 64) == 0
+    assert lib.cr_mx4_rows(BASE, 0, 192, 3, _mx4(capi, inner=192), workspace, need - short, out, 1, None) == capi.ERR_INVALID
 
 
 def test_operands_of_different_inner_size(capi):
