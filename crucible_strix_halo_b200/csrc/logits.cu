@@ -1,10 +1,12 @@
 // Penalties, biases and grammar masks on the logits of spans, and the greedy choice (see cr_logits_choose for the formula).
 // Every product, quotient and sum is rounded by itself (no contraction), so that a choice is the definition's own.
 //
-// HBM-bound with many rows, latency-bound with one: a cluster of eight CTAs takes some rows of a span, its warps 256 tokens at a time in
-// eight runs of 32, so that rows of any pitch and address are read a line at a time.  Counts and biases are read once for all rows
-// of the cluster; a draft raises its token's count from the next row on.  The best token of a row goes from thread to warp to CTA, and
-// the CTAs' are gathered through distributed shared memory: one launch, no scratch.
+// HBM-bound with many rows, latency-bound with one: a cluster of eight CTAs takes a row, its warps 256 tokens at a time in eight runs of
+// 32, so that rows of any pitch and address are read a line at a time, the next 256 while these are worked on.  Counts and biases
+// come from L2 after the first row.  The division by the repetition penalty is left to the runs that hold a repeated token.  The best
+// token goes from thread to warp to CTA, and the CTAs' are gathered through distributed shared memory: one launch, no scratch.
+// All rows of a span in one cluster, with counts, biases and keys of twelve rows in registers, took 90 us for 8 x 9 rows of 100,352
+// (87 instructions a token, a sixth of the time waiting for them to be fetched).
 #include <cooperative_groups.h>
 #include "mx4.cuh"
 
@@ -13,7 +15,6 @@ namespace cg = cooperative_groups;
 namespace cr {
 
 constexpr int kChooseCluster = 8;
-constexpr int kChooseRows = 12;                    // rows of a span that a cluster takes at most
 
 struct LogitsTable { cr_logits_args s[kMaxSpans]; };
 
@@ -23,113 +24,156 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 
-__device__ __forceinline__ float processed(float l, int n, float bias, const cr_logits_args& a) {
-  if (n > 0) {
-    l = l > 0.f ? __fdiv_rn(l, a.repetition) : __fmul_rn(l, a.repetition);
-    l = __fsub_rn(__fsub_rn(l, __fmul_rn((float)n, a.frequency)), a.presence);
-  }
-  return a.bias ? __fadd_rn(l, bias) : l;
-}
-
 template <int TYPE>
-__device__ __forceinline__ float load_logit(const void* p, size_t i) {
-  if constexpr (TYPE == CR_ROW_F32) return __ldcs(reinterpret_cast<const float*>(p) + i);
-  else if constexpr (TYPE == CR_ROW_BF16) return bf16_bits_to_float(__ldcs(reinterpret_cast<const unsigned short*>(p) + i));
-  else return __half2float(__ushort_as_half(__ldcs(reinterpret_cast<const unsigned short*>(p) + i)));
+__device__ __forceinline__ uint32_t logit_bits(const char* p) {
+  if constexpr (TYPE == CR_ROW_F32) return __ldcs(reinterpret_cast<const unsigned*>(p));
+  else return __ldcs(reinterpret_cast<const unsigned short*>(p));
+}
+template <int TYPE>
+__device__ __forceinline__ float logit_value(uint32_t u) {
+  if constexpr (TYPE == CR_ROW_F32) return __uint_as_float(u);
+  else if constexpr (TYPE == CR_ROW_BF16) return __uint_as_float(u << 16);
+  else return __half2float(__ushort_as_half((unsigned short)u));
 }
 
-// Rows r0 .. r0 + n - 1 of a span, the tokens of this CTA; the best of every warp to warp_best[warp][row]: key and complement of the
-// index, so that the larger number is the better token and the lower index among equals.  0: none allowed.
-template <int TYPE, int ROWS, int THREADS>
-__device__ __forceinline__ void choose_rows(const cr_logits_args& a, int r0, int n, int rank, uint64_t (*warp_best)[ROWS]) {
-  const int t = threadIdx.x, l = t & 31, warp = rank * (THREADS / 32) + (t >> 5);
-  uint32_t key[ROWS];
-  int at[ROWS];
+// What a warp has found: key and index of its lanes' best tokens.
+struct Best { uint32_t key = 0; int at = 0; };
+
+// 256 tokens from v0 on; FULL: all of them below V.
+template <bool FULL>
+__device__ __forceinline__ void choose_piece(const cr_logits_args& a, int r, int v0, float (&x)[8], const uint32_t* mask, float* out, Best& best) {
+  const int l = threadIdx.x & 31;
+  int n[8];
+  bool said = false;
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) { key[r] = 0; at[r] = 0; }
-  const int earlier = a.drafts ? r0 : 0;
-  for (int v0 = warp * 256; v0 < a.V; v0 += kChooseCluster * (THREADS / 32) * 256) {
-    int count[8];
-    float bias[8];
+  for (int k = 0; k < 8; ++k) n[k] = 0;
+  if (a.counts) {
+    const int* p = a.counts + v0 + l;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) n[k] = FULL || v0 + 32 * k + l < a.V ? p[32 * k] : 0;
+  }
+  uint32_t word = 0xffffffffu;                                            // lane k < 8 has the words of run k
+  if (mask && l < 8 && (FULL || v0 + 32 * l < a.V)) word = mask[(v0 >> 5) + l];
+  if (a.drafts)
+    for (int j = 0; j < r; ++j) {
+      const int d = a.drafts[j] - v0;
+      if ((unsigned)d < 256u) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) n[k] += d == 32 * k + l;
+      }
+    }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) said |= n[k] > 0;
+  if (__any_sync(0xffffffffu, said)) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (n[k] > 0) {
+        x[k] = x[k] > 0.f ? __fdiv_rn(x[k], a.repetition) : __fmul_rn(x[k], a.repetition);
+        x[k] = __fsub_rn(__fsub_rn(x[k], __fmul_rn((float)n[k], a.frequency)), a.presence);
+      }
+  }
+  if (a.bias) {
+    const float* p = a.bias + v0 + l;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = __fadd_rn(x[k], FULL || v0 + 32 * k + l < a.V ? p[32 * k] : 0.f);
+  }
+  if (mask) {
+    uint32_t mine = 0;                                                    // bit k: token 32 k + l is allowed
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mine |= (__shfl_sync(0xffffffffu, word, k) >> l & 1) << k;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int v = v0 + 32 * k + l;
-      count[k] = a.counts && v < a.V ? a.counts[v] : 0;
-      bias[k] = a.bias && v < a.V ? a.bias[v] : 0.f;
+      const bool allowed = mine >> k & 1;
+      const uint32_t o = order_key(x[k]);
+      x[k] = allowed ? x[k] : -INFINITY;
+      if (allowed && (FULL || v0 + 32 * k + l < a.V) && o > best.key) { best.key = o; best.at = v0 + 32 * k + l; }
     }
-    for (int j = 0; j < earlier; ++j) {
-      const int d = a.drafts[j] - v0 - l;
+  } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) count[k] += d == 32 * k;
-    }
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      if (r >= n) break;
-      float x[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int v = v0 + 32 * k + l;
-        x[k] = v < a.V ? load_logit<TYPE>(a.logits, (size_t)(r0 + r) * a.ld + v) : 0.f;
-      }
-      // lane k < 8 has the words of the piece
-      uint32_t word = 0xffffffffu;
-      if (a.mask && l < 8 && v0 + 32 * l < a.V) word = a.mask[(size_t)(r0 + r) * a.mask_ld + (v0 >> 5) + l];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int v = v0 + 32 * k + l;
-        const bool allowed = (__shfl_sync(0xffffffffu, word, k) >> l & 1) && v < a.V;
-        const float y = processed(x[k], count[k], bias[k], a);
-        const uint32_t o = order_key(y);
-        if (allowed && o > key[r]) { key[r] = o; at[r] = v; }
-        if (a.out && v < a.V) __stcs(a.out + (size_t)(r0 + r) * a.out_ld + v, allowed ? y : -INFINITY);
-      }
-      if (a.drafts && r + 1 < n) {                                  // the row's draft counts from the next row on
-        const int d = a.drafts[r0 + r] - v0 - l;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) count[k] += d == 32 * k;
-      }
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t o = order_key(x[k]);
+      if ((FULL || v0 + 32 * k + l < a.V) && o > best.key) { best.key = o; best.at = v0 + 32 * k + l; }
     }
   }
+  if (out) {
+    float* p = out + v0 + l;
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    if (r >= n) break;
-    const uint32_t top = __reduce_max_sync(0xffffffffu, key[r]);
-    const uint32_t low = __reduce_min_sync(0xffffffffu, key[r] == top ? (uint32_t)at[r] : 0xffffffffu);
-    if (l == 0) warp_best[t >> 5][r] = top ? (uint64_t)top << 32 | ~low : 0;
+    for (int k = 0; k < 8; ++k)
+      if (FULL || v0 + 32 * k + l < a.V) __stcs(p + 32 * k, x[k]);
   }
 }
 
-// grid: (8 CTAs x row groups, spans).
-template <int ROWS, int THREADS>
-__global__ void __cluster_dims__(kChooseCluster, 1, 1) __launch_bounds__(THREADS)
-logits_choose_kernel(const __grid_constant__ LogitsTable T, int group_rows) {
-  __shared__ uint64_t warp_best[THREADS / 32][ROWS], cta_best[ROWS];
+// Row r, the tokens of this warp out of `warps`.  Returns the warp's best: key and complement of the index, so that the larger number
+// is the better token and the lower index among equals; 0 where none is allowed.
+template <int TYPE>
+__device__ __forceinline__ uint64_t choose_row(const cr_logits_args& a, int r, int warp, int warps) {
+  constexpr int SIZE = TYPE == CR_ROW_F32 ? 4 : 2;
+  const int l = threadIdx.x & 31, step = warps * 256;
+  const char* row = static_cast<const char*>(a.logits) + ((size_t)r * a.ld + l) * SIZE;
+  float* out = a.out ? a.out + (size_t)r * a.out_ld : nullptr;
+  const uint32_t* mask = a.mask ? a.mask + (size_t)r * a.mask_ld : nullptr;
+  Best best;
+  uint32_t ahead[8];
+  auto fetch = [&](int v0) {
+    const char* p = row + (size_t)v0 * SIZE;
+    if (v0 + 256 <= a.V) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) ahead[k] = logit_bits<TYPE>(p + 32 * k * SIZE);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) ahead[k] = v0 + 32 * k + l < a.V ? logit_bits<TYPE>(p + 32 * k * SIZE) : 0;
+    }
+  };
+  if (warp * 256 < a.V) fetch(warp * 256);
+#pragma unroll 1
+  for (int v0 = warp * 256; v0 < a.V; v0 += step) {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = logit_value<TYPE>(ahead[k]);
+    if (v0 + step < a.V) fetch(v0 + step);
+    if (v0 + 256 <= a.V) choose_piece<true>(a, r, v0, x, mask, out, best);
+    else choose_piece<false>(a, r, v0, x, mask, out, best);
+  }
+  const uint32_t top = __reduce_max_sync(0xffffffffu, best.key);
+  const uint32_t low = __reduce_min_sync(0xffffffffu, best.key == top ? (uint32_t)best.at : 0xffffffffu);
+  return top ? (uint64_t)top << 32 | (uint32_t)~low : 0;
+}
+
+// grid: (8 CTAs x rows, spans).
+template <int THREADS>
+__global__ void __cluster_dims__(kChooseCluster, 1, 1) __launch_bounds__(THREADS, 1024 / THREADS) logits_choose_kernel(const __grid_constant__ LogitsTable T) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ uint64_t warp_best[WARPS], cta_best[kChooseCluster];
   cg::cluster_group cluster = cg::this_cluster();
+  cluster.barrier_arrive();                                             // this CTA's shared memory may be written from now on
   const cr_logits_args& a = T.s[blockIdx.y];
-  const int rank = (int)cluster.block_rank(), t = threadIdx.x;
-  const int r0 = blockIdx.x / kChooseCluster * group_rows, n = min(group_rows, a.R - r0);
+  const int rank = (int)cluster.block_rank(), t = threadIdx.x, r = blockIdx.x / kChooseCluster, warp = rank * WARPS + (t >> 5);
   pdl_release();
   pdl_wait();
-  if (n <= 0) return;                                                // the same for the whole cluster
-  if (a.dtype == CR_ROW_F32) choose_rows<CR_ROW_F32, ROWS, THREADS>(a, r0, n, rank, warp_best);
-  else if (a.dtype == CR_ROW_BF16) choose_rows<CR_ROW_BF16, ROWS, THREADS>(a, r0, n, rank, warp_best);
-  else choose_rows<CR_ROW_F16, ROWS, THREADS>(a, r0, n, rank, warp_best);
-  if (!a.choice) return;
+  uint64_t best = 0;
+  if (r < a.R) {
+    if (a.dtype == CR_ROW_F32) best = choose_row<CR_ROW_F32>(a, r, warp, kChooseCluster * WARPS);
+    else if (a.dtype == CR_ROW_BF16) best = choose_row<CR_ROW_BF16>(a, r, warp, kChooseCluster * WARPS);
+    else best = choose_row<CR_ROW_F16>(a, r, warp, kChooseCluster * WARPS);
+  }
+  if ((t & 31) == 0) warp_best[t >> 5] = best;
   __syncthreads();
-  for (int r = t >> 5; r < n; r += THREADS / 32) {                    // a warp per row
-    uint64_t best = (t & 31) < THREADS / 32 ? warp_best[t & 31][r] : 0;
+  cluster.barrier_wait();
+  if (t < 32) {                                                         // the CTA's best to the first CTA of the cluster
+    best = t < WARPS ? warp_best[t] : 0;
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, m));
-    if ((t & 31) == 0) cta_best[r] = best;
+    if (t == 0) *cluster.map_shared_rank(&cta_best[rank], 0) = best;
   }
-  cluster.sync();
-  if (rank == 0 && t < n) {
-    uint64_t best = 0;
+  cluster.barrier_arrive();
+  if (rank != 0) return;                                                // arrived: nobody writes here
+  cluster.barrier_wait();
+  if (t < 32 && r < a.R) {
+    best = t < kChooseCluster ? cta_best[t] : 0;
 #pragma unroll
-    for (int k = 0; k < kChooseCluster; ++k) best = max(best, *cluster.map_shared_rank(&cta_best[t], k));
-    a.choice[r0 + t] = best ? (int)~(uint32_t)best : -1;
+    for (int m = kChooseCluster / 2; m > 0; m >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, m));
+    if (t == 0 && a.choice) a.choice[r] = best ? (int)~(uint32_t)best : -1;
   }
-  cluster.sync();                                                    // a CTA stays until its best tokens have been read
 }
 
 __global__ void __launch_bounds__(256) token_count_kernel(const int* __restrict__ tokens, int n, int delta, int* counts, int V) {
@@ -148,7 +192,7 @@ extern "C" cr_status cr_logits_choose(const cr_logits_args* spans, int n_spans, 
   CR_REQUIRE(spans && n_spans >= 1, "cr_logits_choose: no spans");
   for (int i = 0; i < n_spans; ++i) {
     const cr_logits_args& a = spans[i];
-    CR_REQUIRE(a.R >= 1 && a.V >= 1, "cr_logits_choose: span %d: R=%d V=%d", i, a.R, a.V);
+    CR_REQUIRE(a.R >= 1 && a.R < (1 << 20) && a.V >= 1 && a.V < (1 << 30), "cr_logits_choose: span %d: R=%d V=%d", i, a.R, a.V);
     if (cr_status s = check_rows(a.logits, a.dtype, a.ld, a.V, "cr_logits_choose")) return s;
     CR_REQUIRE(a.out || a.choice, "cr_logits_choose: span %d asks for nothing", i);
     CR_REQUIRE(!a.out || a.out_ld >= a.V, "cr_logits_choose: span %d: pitch %lld of the processed logits below V=%d", i, a.out_ld, a.V);
@@ -164,12 +208,9 @@ extern "C" cr_status cr_logits_choose(const cr_logits_args* spans, int n_spans, 
     const int n = n_spans - i0 < kMaxSpans ? n_spans - i0 : kMaxSpans;
     int rows = 1;
     for (int i = 0; i < n; ++i) { T.s[i] = spans[i0 + i]; rows = rows > T.s[i].R ? rows : T.s[i].R; }
-    // One row per cluster while all clusters run at once, else as many rows as that takes: the counts and biases are read once for them.
-    const int room = sm_count() / kChooseCluster / n, want = room > 0 ? (rows + room - 1) / room : rows;
-    const int group = want < kChooseRows ? want : kChooseRows;
-    const dim3 grid((unsigned)(kChooseCluster * ((rows + group - 1) / group)), n);
-    if (group == 1) CR_CUDA(launch_pdl(logits_choose_kernel<1, 1024>, grid, dim3(1024), 0, stream, T, group));
-    else CR_CUDA(launch_pdl(logits_choose_kernel<kChooseRows, 512>, grid, dim3(512), 0, stream, T, group));
+    const dim3 grid((unsigned)(kChooseCluster * rows), n);
+    if (rows * n * kChooseCluster <= sm_count()) CR_CUDA(launch_pdl(logits_choose_kernel<1024>, grid, dim3(1024), 0, stream, T));
+    else CR_CUDA(launch_pdl(logits_choose_kernel<512>, grid, dim3(512), 0, stream, T));
     CR_LAUNCH_CHECK("logits_choose_kernel");
   }
   return CR_OK;
