@@ -194,16 +194,12 @@ class Mx4:
 
 def mx4_quant(x, out=None):
     """Rows x [rows, inner] (float32, bfloat16 or float16, any row pitch) as an Mx4 (cr_mx4_quant)."""
-    if out is None:
-        if x.dim() != 2:
-            raise ValueError("x must be a matrix")
-        out = Mx4.empty(x.shape[0], x.shape[1], x.device)
-    return _binding.mx4_quant(x, out)
+    return _binding.mx4_quant(x, Mx4 if out is None else out)
 
 
 def mx4_dequant(m, dtype=torch.float32, out=None):
     """The numbers an Mx4 stands for, as rows of `dtype` (cr_mx4_dequant)."""
-    return _binding.mx4_dequant(m, torch.empty(m.rows, m.inner, device=m.codes.device, dtype=dtype) if out is None else out)
+    return _binding.mx4_dequant(m, dtype if out is None else out)
 
 
 def mx4_gemm(x, w, outs):

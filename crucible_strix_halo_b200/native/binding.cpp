@@ -2,6 +2,7 @@
 // attributes; through ctypes that, the stream look-up and the outputs took 15 us per GDN call and 24 us per QSA call, three
 // times their launches.  Here the same objects (weights, sessions, plans, span dicts) are read with the CPython API and the
 // argument structs of include/crucible_attn.h are filled on the stack.
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
@@ -382,36 +383,57 @@ std::vector<cr_proj_out> projections(PyObject* outs, int64_t rows) {
   return o;
 }
 
-PyObject* mx4_quant(PyObject*, PyObject* args) {     // (x, to)
+PyObject* mx4_quant(PyObject*, PyObject* args) {     // (x, to, or the class of a new matrix)
   return guarded([&]() -> PyObject* {
     PyObject *x, *to;
     if (!PyArg_ParseTuple(args, "OO", &x, &to)) throw Error();
     const at::Tensor& xt = here(x, "x");
     const cr_row_dtype type = row_type(xt, "x");
     const int64_t ld = pitch(xt, "x");
-    const cr_mx4 m = mx4(to, "the 4-bit matrix");
-    if (xt.size(0) != m.rows || xt.size(1) != m.inner) refuse(PyExc_ValueError, "%s has another shape than the 4-bit matrix", "x");
+    cr_mx4 m{};
+    PyObject* out = nullptr;
+    if (PyType_Check(to)) {
+      m.rows = count(xt.size(0), "x");
+      m.inner = count(xt.size(1), "x");
+      if (m.rows < 1 || m.inner < 64 || m.inner % 64) refuse(PyExc_ValueError, "%s", "a 4-bit matrix has at least one row and a multiple of 64 elements in it");
+      const auto bytes = at::TensorOptions().dtype(at::kByte).device(xt.device());
+      const at::Tensor codes = at::empty({m.rows, m.inner / 2}, bytes);
+      const at::Tensor scales = at::empty({((int64_t)m.rows + 127) / 128 * (((int64_t)m.inner + 127) / 128) * 512}, bytes);
+      m.codes = codes.data_ptr<uint8_t>();
+      m.scales = scales.data_ptr<uint8_t>();
+      Ref c(wrap(codes)), s(wrap(scales));
+      out = PyObject_CallFunction(to, "OOii", c.p, s.p, m.rows, m.inner);
+      if (!out) throw Error();
+    } else {
+      m = mx4(to, "the 4-bit matrix");
+      if (xt.size(0) != m.rows || xt.size(1) != m.inner) refuse(PyExc_ValueError, "%s has another shape than the 4-bit matrix", "x");
+      Py_INCREF(to);
+      out = to;
+    }
+    Ref held(out);
     const void* const xp = xt.data_ptr();
     void* const st = stream();
     check(unlocked([&] { return present(cr_mx4_quant)(xp, type, ld, &m, st); }));
-    Py_INCREF(to);
-    return to;
+    Py_INCREF(out);
+    return out;
   });
 }
 
-PyObject* mx4_dequant(PyObject*, PyObject* args) {   // (m, out)
+PyObject* mx4_dequant(PyObject*, PyObject* args) {   // (m, out, or the type of new rows)
   return guarded([&]() -> PyObject* {
-    PyObject *from, *out;
-    if (!PyArg_ParseTuple(args, "OO", &from, &out)) throw Error();
+    PyObject *from, *to;
+    if (!PyArg_ParseTuple(args, "OO", &from, &to)) throw Error();
     const cr_mx4 m = mx4(from, "the 4-bit matrix");
+    Ref out(THPDtype_Check(to) ? wrap(at::empty({m.rows, m.inner}, at::TensorOptions().dtype(reinterpret_cast<THPDtype*>(to)->scalar_type).device(at::kCUDA)))
+                               : (Py_INCREF(to), to));
     const at::Tensor& t = here(out, "out");
     const cr_row_dtype type = row_type(t, "out");
     const int64_t ld = pitch(t, "out");
     if (t.size(0) != m.rows || t.size(1) != m.inner) refuse(PyExc_ValueError, "%s has another shape than the 4-bit matrix", "out");
     void *const p = t.data_ptr(), *const st = stream();
     check(unlocked([&] { return present(cr_mx4_dequant)(&m, p, type, ld, st); }));
-    Py_INCREF(out);
-    return out;
+    Py_INCREF(out.p);
+    return out.p;
   });
 }
 
