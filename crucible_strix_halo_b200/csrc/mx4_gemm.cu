@@ -21,77 +21,65 @@ namespace cr {
 CR_DEFINE_STATUS_WORD(mx4_gemm)
 
 // ---- epilogue: rows of a warp's 32 accumulator lanes to the outputs -----------------------------------------------------
-// A lane holds a row; stored from there, an instruction would touch 32 lines for 512 bytes.  The warp turns its rows through 4 KB of
-// shared memory (16-byte chunks exchanged by row, free of bank conflicts) and stores 128 or 64 bytes of a row at a time.
-// N16: 16-byte chunks of a row.
-template <int N16>
-__device__ __forceinline__ void store_turned(unsigned char* buf, const uint4 (&v)[N16], char* to, size_t pitch, int live) {
+// A lane holds a row; stored from there, an instruction would touch 32 lines for 512 bytes.  The warp turns its rows through 2 KB of
+// shared memory, 64 bytes of every row at a time (16-byte chunks exchanged by row, free of bank conflicts).
+constexpr int kTurnBytes = 2048;
+__device__ __forceinline__ void store_turned(unsigned char* buf, const uint4 (&v)[4], char* to, size_t pitch, int live) {
   const int l = threadIdx.x & 31;
 #pragma unroll
-  for (int c = 0; c < N16; ++c) *reinterpret_cast<uint4*>(buf + l * 128 + ((c ^ (l & 7)) << 4)) = v[c];
+  for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(buf + l * 64 + ((c ^ (l >> 1 & 3)) << 4)) = v[c];
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < N16; ++i) {
-    const int r = i * (32 / N16) + l / N16, c = l % N16;
-    if (r < live) *reinterpret_cast<uint4*>(to + r * pitch + c * 16) = *reinterpret_cast<const uint4*>(buf + r * 128 + ((c ^ (r & 7)) << 4));
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + l / 4, c = l % 4;
+    if (r < live) *reinterpret_cast<uint4*>(to + r * pitch + c * 16) = *reinterpret_cast<const uint4*>(buf + r * 64 + ((c ^ (r >> 1 & 3)) << 4));
   }
   __syncwarp();
 }
-template <int N16>
-__device__ __forceinline__ void pack_bf16(uint4 (&p)[N16], const float* v) {
+// Columns col .. col + 31 (which no output divides) of `live` rows from row0 on.
+__device__ __forceinline__ void store_columns(const ProjParams& P, unsigned char* buf, int row0, int col, const float (&v)[32], int live) {
+  int o = 0;
+  while (o < P.n_outs - 1 && col >= P.col0[o] + P.cols[o]) ++o;
+  const size_t at = (size_t)row0 * P.ld[o] + (col - P.col0[o]), pitch = P.ld[o];
+  uint4 p[4];
+  if (P.f32[o]) {
 #pragma unroll
-  for (int c = 0; c < N16; ++c) {
-    unsigned k[4];
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const __nv_bfloat162 b2 = __floats2bfloat162_rn(v[8 * c + 2 * j], v[8 * c + 2 * j + 1]);
-      k[j] = *reinterpret_cast<const unsigned*>(&b2);
+      for (int c = 0; c < 4; ++c) {
+        const float* f = v + 16 * h + 4 * c;
+        p[c] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+      }
+      store_turned(buf, p, reinterpret_cast<char*>(reinterpret_cast<float*>(P.ptr[o]) + at + 16 * h), pitch * 4, live);
     }
-    p[c] = make_uint4(k[0], k[1], k[2], k[3]);
-  }
-}
-// Columns col .. col + 32 CH - 1 (CH: 1 or 2 chunks that an output does not divide) of `live` rows from row0 on.
-template <int CH>
-__device__ __forceinline__ void store_columns(const ProjParams& P, unsigned char* buf, int row0, int col, const float (&v)[32 * CH], int live) {
-  int o[CH];
+  } else {
 #pragma unroll
-  for (int k = 0; k < CH; ++k) {
-    o[k] = 0;
-    while (o[k] < P.n_outs - 1 && col + 32 * k >= P.col0[o[k]] + P.cols[o[k]]) ++o[k];
-  }
-  auto place = [&](int k, int size) { return reinterpret_cast<char*>(P.ptr[o[k]]) + ((size_t)row0 * P.ld[o[k]] + (col + 32 * k - P.col0[o[k]])) * size; };
-  if (CH == 2 && o[0] == o[CH - 1] && !P.f32[o[0]] && col + 32 < P.N) {
-    uint4 p[4 * CH];
-    pack_bf16(p, v);
-    store_turned(buf, p, place(0, 2), (size_t)P.ld[o[0]] * 2, live);
-    return;
-  }
+    for (int c = 0; c < 4; ++c) {
+      unsigned k[4];
 #pragma unroll
-  for (int k = 0; k < CH; ++k) {
-    if (col + 32 * k >= P.N) return;
-    if (P.f32[o[k]]) {
-      store_turned(buf, reinterpret_cast<const uint4(&)[8]>(v[32 * k]), place(k, 4), (size_t)P.ld[o[k]] * 4, live);
-    } else {
-      uint4 p[4];
-      pack_bf16(p, v + 32 * k);
-      store_turned(buf, p, place(k, 2), (size_t)P.ld[o[k]] * 2, live);
+      for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 b2 = __floats2bfloat162_rn(v[8 * c + 2 * j], v[8 * c + 2 * j + 1]);
+        k[j] = *reinterpret_cast<const unsigned*>(&b2);
+      }
+      p[c] = make_uint4(k[0], k[1], k[2], k[3]);
     }
+    store_turned(buf, p, reinterpret_cast<char*>(reinterpret_cast<__nv_bfloat16*>(P.ptr[o]) + at), pitch * 2, live);
   }
 }
 
 // ---- CTA pairs on 256 x 256 tiles ------------------------------------------------------------------------------------
 constexpr int kQStages = 5, kQStageBytes = 2 * kXTile + 3 * kXScale, kQBand = 16;
-constexpr int kQThreads = 64 + 256;                                       // producer, issuer, eight epilogue warps
+constexpr int kQWarps = 16, kQThreads = 64 + 32 * kQWarps;                // producer, issuer, epilogue warps
 constexpr int kQShared = 128, kQScaleCols = 512 - kQShared;               // columns that both accumulators use; first scale column
 static_assert(kQStages * 24 <= kQShared, "every stage has scale columns of its own");
-constexpr int kQTurn = kQStages * kQStageBytes;                            // 4 KB for each epilogue warp behind the stages
-constexpr size_t kQSmem = (size_t)kQTurn + 8 * 4096 + (2 * kQStages + 4) * 8 + 16;
+constexpr int kQTurn = kQStages * kQStageBytes;                            // room of the epilogue warps behind the stages
+constexpr size_t kQSmem = (size_t)kQTurn + kQWarps * kTurnBytes + (2 * kQStages + 4) * 8 + 16;
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kQThreads, 1)
 mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
                      const __grid_constant__ CUtensorMap xsmap, const __grid_constant__ CUtensorMap wsmap) {
   extern __shared__ __align__(1024) unsigned char sm[];
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kQTurn + 8 * 4096);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kQTurn + kQWarps * kTurnBytes);
   uint64_t *full = bars, *empty = bars + kQStages, *accFull = bars + 2 * kQStages, *handed = bars + 2 * kQStages + 2;
   uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 2 * kQStages + 4);
   volatile int& dead = *reinterpret_cast<volatile int*>(&tmem_slot + 1);
@@ -109,7 +97,7 @@ mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant
   if (t == 0) {
     for (int i = 0; i < kQStages; ++i) { umma::mbar_init(&full[i], 1); umma::mbar_init(&empty[i], 1); }
     for (int i = 0; i < 2; ++i) umma::mbar_init(&accFull[i], 1);
-    umma::mbar_init(handed, 16);                                          // eight epilogue warps in each CTA
+    umma::mbar_init(handed, 2 * kQWarps);                                 // the epilogue warps of both CTAs
     umma::mbar_fence_init();
     dead = (umma::smem_u32(sm) & 1023u) != 0;                           // the swizzled tiles need 1 KB boundaries
     if (dead) g_mx4_gemm_status = 1;
@@ -176,7 +164,7 @@ mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant
       }
     }
   } else {
-    // ---------------------------------------------------------------- epilogue: two warps to each quarter of the lanes
+    // ---------------------------------------------------------------- epilogue: four warps to each quarter of the lanes
     const int q = w & 3, h = (w - 2) >> 2;
     int local = 0;
     for (int i = pair; i < tiles; i += pairs, ++local) {
@@ -188,18 +176,18 @@ mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant
       if (dead) break;
       umma::fence_after_sync();
       const int row0 = m0 + 128 * (int)rank + 32 * q, live = min(32, P.R - row0);
-#pragma unroll 1
+#pragma unroll
       for (int j = 0; j < 2; ++j) {
-        // 64 columns at a time; the shared ones are the last half of the even accumulator and the first half of the odd one
-        const int c = ((odd + j) & 1 ? 0 : 4) + 2 * h;
-        float v[64];
-        umma::tmem_ld64(umma::tmem_addr(tm, q, odd * (256 - kQShared) + 32 * c), v);     // warp-collective
+        // the shared columns are the last half of the even accumulator and the first half of the odd one
+        const int c = ((odd + j) & 1 ? 0 : 4) + h;
+        float v[32];
+        umma::tmem_ld32(umma::tmem_addr(tm, q, odd * (256 - kQShared) + 32 * c), v);     // warp-collective
         if (j == 0) {
           umma::fence_before_sync();
           __syncwarp();
           if (l == 0) umma::pair_arrive_relaxed(umma::cluster_addr(handed, 0));
         }
-        if (live > 0 && n0 + 32 * c < P.N) store_columns<2>(P, sm + kQTurn + (w - 2) * 4096, row0, n0 + 32 * c, v, live);
+        if (live > 0 && n0 + 32 * c < P.N) store_columns(P, sm + kQTurn + (w - 2) * kTurnBytes, row0, n0 + 32 * c, v, live);
       }
     }
   }
@@ -302,7 +290,7 @@ mx4_gemm_split_kernel(const __grid_constant__ ProjParams P, const __grid_constan
         umma::tmem_ld32(umma::tmem_addr(tm, q, 32 * c), v);                 // warp-collective
         if (splits == 1) {
           const int row0 = m0 + 32 * q;                                     // the stages have been read: their place serves to turn the rows
-          if (row0 < P.R && n0 + 32 * c < P.N) store_columns<1>(P, sm + (w - 2) * 4096, row0, n0 + 32 * c, v, min(32, P.R - row0));
+          if (row0 < P.R && n0 + 32 * c < P.N) store_columns(P, sm + (w - 2) * kTurnBytes, row0, n0 + 32 * c, v, min(32, P.R - row0));
         } else {                                                            // the stages have been read: the partial tile goes over them
           float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(sm) + (size_t)r * kVLd<TN> + 32 * c);
 #pragma unroll
