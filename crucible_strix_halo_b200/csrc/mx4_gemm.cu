@@ -1,15 +1,13 @@
 // Product of two matrices of microscaled 4-bit floats for sm_100a: Y[R][N] = X[R][K] W[N][K]^T, fp32 accumulation, the columns
 // scattered into the outputs as cr_proj_gemm does (mx4_mma.cuh: how the operands and scales reach the tensor cores).
 //
-// A step moves the bytes of a bf16 step of 16 (4 bits against 16, four times as many), in the same cycles, so the cuts are those of
-// cr_proj_gemm with K / 4 in the place of K.
+// A step of 64 moves the bytes of a bf16 step of 16 in the same cycles, so the kernels are shaped as those of cr_proj_gemm.
 //
 // mx4_gemm_pair_kernel (many rows): CTA pairs on 256 x 256 tiles.  Two accumulators of 256 columns would fill tensor memory and
-// leave the scales no room: they share 64 columns, which the epilogue reads first and hands over before it stores.
+// leave the scales no room: they share 128 columns, which the epilogue reads first and hands over before it stores.
 // mx4_gemm_split_kernel<TN> (few rows): 128 x TN tiles, K split over a cluster of up to eight CTAs.
 //
-// The scale columns of tensor memory have two buffers.  tcgen05.cp is ordered before the products issued after it, but not behind
-// those issued before it: the issuer waits until the products of the stage before the last have completed.
+// Every stage has scale columns of its own in tensor memory: they are free when the stage is.
 // Every wait is bounded; a wait that gives up raises bit 5 of the device status word.
 #include <cooperative_groups.h>
 #include "mx4_mma.cuh"
@@ -206,7 +204,7 @@ constexpr size_t kVSmem = (size_t)kVRing + (2 * kVMaxStages + 1) * 8 + 16;
 constexpr int kVThreads = 64 + 256;
 template <int TN> constexpr int kVGroups = TN > 128 ? 2 : 1;             // row groups of W's scales
 template <int TN> constexpr int kVScaleCols = 8 + 8 * kVGroups<TN>;
-template <int TN> constexpr int kVCols = TN + 2 * kVScaleCols<TN> <= 128 ? 128 : (TN + 2 * kVScaleCols<TN> <= 256 ? 256 : 512);
+template <int TN> constexpr int kVStages = (512 - TN) / kVScaleCols<TN> < kVMaxStages ? (512 - TN) / kVScaleCols<TN> : kVMaxStages;   // as many as have scale columns
 
 // grid: tiles x splits, cluster = splits (along x).
 template <int TN>
@@ -233,7 +231,7 @@ mx4_gemm_split_kernel(const __grid_constant__ ProjParams P, const __grid_constan
     if (dead) g_mx4_gemm_status = 1;
     prefetch_map(&xmap); prefetch_map(&wmap); prefetch_map(&xsmap); prefetch_map(&wsmap);
   }
-  if (w == 1) umma::tmem_alloc(&tmem_slot, kVCols<TN>);
+  if (w == 1) umma::tmem_alloc(&tmem_slot, 512);
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
@@ -264,11 +262,10 @@ mx4_gemm_split_kernel(const __grid_constant__ ProjParams P, const __grid_constan
     const Desc xc(tma::desc_sw128(sm, 16, 1024)), wc(tma::desc_sw128(sm + xbytes, 16, 1024));
     const Desc xs(umma::smem_desc(sm + xbytes + TN * (kXK / 2), 0, 128)), ws(umma::smem_desc(sm + xbytes + TN * (kXK / 2) + kXScale, 0, 128));
     for (int it = 0, s = 0, phase = 0; it < kb_n; ++it) {
-      if (it >= 2) wait(&empty[(it - 2) % ST], ((it - 2) / ST) & 1);       // the scale columns' last readers are done
       wait(&full[s], phase);
       if (gave_up) break;
       umma::fence_after_sync();
-      const uint32_t off = s * (stage / 16), cols = tm + TN + (it & 1) * kVScaleCols<TN>;
+      const uint32_t off = s * (stage / 16), cols = tm + TN + s * kVScaleCols<TN>;
       const int steps = P.K / 64 - (kb0 + it) * 4;
       if (one) {
         issue_scales<1, NG>(cols, xs, ws, off, steps);
@@ -301,7 +298,7 @@ mx4_gemm_split_kernel(const __grid_constant__ ProjParams P, const __grid_constan
   }
   umma::fence_before_sync();
   __syncthreads();
-  if (w == 1) umma::tmem_dealloc(tm, kVCols<TN>);
+  if (w == 1) umma::tmem_dealloc(tm, 512);
   if (splits == 1) return;
   // Every CTA of the cluster sums a slice of the rows over all partial tiles, in the order of K.
   cg::cluster_group cluster = cg::this_cluster();
@@ -335,8 +332,11 @@ mx4_gemm_split_kernel(const __grid_constant__ ProjParams P, const __grid_constan
   cluster.sync();                                                          // the partial tiles stay until everybody has read them
 }
 
-// How a product is cut: the rule of cr_proj_gemm with steps of 64.  A split has to fit in one wave of the clusters that the device
-// holds at once, which the runtime is asked for.
+// How a product is cut.  Costs in cycles, from eighteen shapes of 1 to 8,192 rows timed with every cut: a step of 64, what a tile takes
+// beside its steps (its first loads and its epilogue; a pair starts later but overlaps them from its second tile on), and the sum over a
+// cluster.  The choice is within 5 % of the fastest cut on all of them (128 x 6,144 x 2,560: 7.7 us on three CTAs a tile of 64 columns,
+// 8.5 on five of 128, 12.9 on pairs; 2,048 x 4,096 x 2,048: 10.6 on 128 x 256, 11.7 on pairs; 4,096 rows: 20.6, 18.2).
+// A split has to fit in one wave of the clusters that the device holds at once, which the runtime is asked for.
 struct Mx4Shape { int tn, splits; };                                       // tn 0: CTA pairs
 static cr_status mx4_cluster_slots(const int (**slots)[9]) {
   static PerDeviceOnce looked_up;
@@ -363,14 +363,14 @@ static Mx4Shape mx4_shape(int R, int K, int N, int sms, const int (&slots)[9]) {
   auto up = [](long long a, long long b) { return (a + b - 1) / b; };
   const long long stages = up(K, kXK);
   Mx4Shape best{0, 1};
-  double cost = (double)up(up(R, 256) * up(N, 256), sms / 2) * up(K, 64) * 133 + 5000;
+  double cost = (double)up(up(R, 256) * up(N, 256), sms / 2) * (up(K, 64) * 125 + 1500) + 9900;
   const int tns[3] = {64, 128, 256};
-  const double step[3] = {96, 132, 195};
+  const double step[3] = {75, 100, 140};
   for (int i = 0; i < 3; ++i) {
     const long long tiles = up(R, kXM) * up(N, tns[i]);
     for (int s = 1; s <= 8 && s <= stages; ++s) {
       if (s > 1 && tiles > slots[s]) break;                                 // splitting pays only while SMs would idle
-      const double c = (double)up(tiles * s, sms) * (up(stages, s) * 4 * step[i] + 3000 + tns[i] * 10 + (s > 1 ? 2500 : 0));
+      const double c = (double)up(tiles * s, sms) * ((s > 1 ? up(stages, s) * 4 : up(K, 64)) * step[i] + 6000 + tns[i] * 10 + (s > 1 ? 500 + tns[i] * 18 : 0));
       if (c < cost) { cost = c; best = Mx4Shape{tns[i], s}; }
     }
   }
@@ -402,7 +402,7 @@ static cr_status mx4_split_launch(const ProjParams& P, const cr_mx4* x, const cr
   }
   cfg.attrs = attr; cfg.numAttrs = na;
   const int stage = (xrows + TN) * (kXK / 2) + (1 + kVGroups<TN>) * kXScale, fit = (kVRing - (stage < kXTile ? kXTile - stage : 0)) / stage;
-  CR_CUDA(cudaLaunchKernelEx(&cfg, mx4_gemm_split_kernel<TN>, P, xmap, wmap, xsmap, wsmap, splits, xrows, fit < kVMaxStages ? fit : kVMaxStages));
+  CR_CUDA(cudaLaunchKernelEx(&cfg, mx4_gemm_split_kernel<TN>, P, xmap, wmap, xsmap, wsmap, splits, xrows, fit < kVStages<TN> ? fit : kVStages<TN>));
   CR_LAUNCH_CHECK("mx4_gemm_split_kernel");
   return CR_OK;
 }
