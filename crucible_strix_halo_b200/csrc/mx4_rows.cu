@@ -89,7 +89,7 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
   const int t = threadIdx.x, w = t >> 5, l = t & 31;
   const int split = blockIdx.x % S.splits, first = blockIdx.x / S.splits, step = gridDim.x / S.splits, units = S.tiles * S.passes;
   const int kb_all = (P.K + kXK - 1) / kXK, kb0 = kb_all * split / S.splits, kb_n = kb_all * (split + 1) / S.splits - kb0;
-  const int xbytes = S.cols * (kXK / 2), ST = S.stages, two = S.cols > 128;
+  const int ST = S.stages, two = S.cols > 128;
   const int accs = two ? 1 : 2, acc_cols = (S.cols + 31) / 32 * 32, scale_cols = two ? 24 : 16;
   if (t == 0) {
     for (int i = 0; i < ST; ++i) { umma::mbar_init(&full[i], 1); umma::mbar_init(&empty[i], 1); }
@@ -113,31 +113,39 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
   // A unit is a tile of W and a pass; the passes of a tile follow one another.  Stage: codes of W, scales of W, codes of X, scales of X.
   if (w == 0) {
     if (l == 0) {
-      const int own = first < units ? (units - first + step - 1) / step : 0, all = own * kb_n;
-      auto load_w = [&](int it) {
-        unsigned char* st = sm + it % ST * S.stage;
-        uint64_t* bar = &full[it % ST];
-        const int n0 = (first + it / kb_n * step) / S.passes * 128, kb = kb0 + it % kb_n;
-        umma::mbar_expect_tx(bar, S.stage);
-        load_box_2d(st, &wmap, kb * (kXK / 2), n0, bar);
-        load_box_2d(st + kXTile, &wsmap, kb * 256, n0 / 128, bar);
+      // Where a stage comes from and goes to, moved on without a division per stage: they set the pace of the copies otherwise.
+      struct Cursor {
+        int unit, left, kb, n0, pass, s = 0, phase = 0;
+        __device__ __forceinline__ void seek(int passes) { n0 = unit / passes; pass = unit - n0 * passes; n0 *= 128; }
       };
-      auto load_x = [&](int it) {
-        unsigned char* st = sm + it % ST * S.stage + kXTile + kXScale;
-        uint64_t* bar = &full[it % ST];
-        const int pass = (first + it / kb_n * step) % S.passes, kb = kb0 + it % kb_n;
-        load_box_2d(st + kXScale * (1 + two), &xmap, kb * (kXK / 2), pass * kPassRows, bar);
-        load_box_2d(st, &xsmap, kb * 256, pass * (kPassRows / 128), bar);
+      const int own = first < units ? (units - first + step - 1) / step : 0;
+      auto begin = [&] { Cursor c; c.unit = first; c.left = own * kb_n; c.kb = 0; c.seek(S.passes); return c; };
+      auto advance = [&](Cursor& c) {
+        --c.left;
+        if (++c.kb == kb_n) { c.kb = 0; c.unit += step; c.seek(S.passes); }
+        if (++c.s == ST) { c.s = 0; c.phase ^= 1; }
       };
-      const int ahead = min(ST, all);
-      for (int it = 0; it < ahead; ++it) load_w(it);
+      auto load_w = [&](const Cursor& c) {
+        unsigned char* st = sm + c.s * S.stage;
+        umma::mbar_expect_tx(&full[c.s], S.stage);
+        load_box_2d(st, &wmap, (kb0 + c.kb) * (kXK / 2), c.n0, &full[c.s]);
+        load_box_2d(st + kXTile, &wsmap, (kb0 + c.kb) * 256, c.n0 / 128, &full[c.s]);
+      };
+      auto load_x = [&](const Cursor& c) {
+        unsigned char* st = sm + c.s * S.stage + kXTile + kXScale;
+        load_box_2d(st + kXScale * (1 + two), &xmap, (kb0 + c.kb) * (kXK / 2), c.pass * kPassRows, &full[c.s]);
+        load_box_2d(st, &xsmap, (kb0 + c.kb) * 256, c.pass * (kPassRows / 128), &full[c.s]);
+      };
+      Cursor cw = begin(), cx = cw;
+      for (int i = 0; i < ST && cw.left > 0; ++i) { load_w(cw); advance(cw); }
       pdl_wait();
-      for (int it = 0; it < ahead; ++it) load_x(it);
-      for (int it = ahead; it < all; ++it) {
-        wait(&empty[it % ST], (it / ST - 1) & 1);
+      for (int i = 0; i < ST && cx.left > 0; ++i) { load_x(cx); advance(cx); }
+      while (cw.left > 0) {
+        wait(&empty[cw.s], cw.phase ^ 1);
         if (gave_up) break;
-        load_w(it);
-        load_x(it);
+        load_w(cw);
+        load_x(cw);
+        advance(cw);
       }
     }
   } else if (w == 1) {
