@@ -152,8 +152,8 @@ mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant
           const uint32_t off = s * (kQStageBytes / 16), cols = tm + kQScaleCols + s * 24;
           const int steps = P.K / 64 - kb * 4;
           if (one) {
-            issue_scales<2, 2>(cols, xs, ws, off, steps);
-            issue_products<2, 2>(acc, xc, wc, off, cols, 0, idesc_mx4(256, 256), steps, kb == 0);
+            issue_scales<2, 2>(cols, xs, off, ws, off, steps);
+            issue_products<2, 2>(acc, xc, off, wc, off, cols, 0, idesc_mx4(256, 256), steps, kb == 0);
             umma::pair_commit(&empty[s]);                                         // the stage is free in both CTAs once these products have read it
             if (kb == kb_n - 1) umma::pair_commit(&accFull[local & 1]);
           }
@@ -268,8 +268,8 @@ mx4_gemm_split_kernel(const __grid_constant__ ProjParams P, const __grid_constan
       const uint32_t off = s * (stage / 16), cols = tm + TN + s * kVScaleCols<TN>;
       const int steps = P.K / 64 - (kb0 + it) * 4;
       if (one) {
-        issue_scales<1, NG>(cols, xs, ws, off, steps);
-        issue_products<1, NG>(tm, xc, wc, off, cols, (n0 & 127) / 32, idesc_mx4(kXM, TN), steps, it == 0);
+        issue_scales<1, NG>(cols, xs, off, ws, off, steps);
+        issue_products<1, NG>(tm, xc, off, wc, off, cols, (n0 & 127) / 32, idesc_mx4(kXM, TN), steps, it == 0);
         umma::commit(&empty[s]);
         if (it == kb_n - 1) umma::commit(accFull);
       }

@@ -60,25 +60,25 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// The scales of one stage: tiles [k group] of X, [row group][k group] of W in shared memory; four columns of tensor memory per tile,
-// those of X first, then W's row groups side by side.
+// The scales of one stage: tiles [k group] of A, [row group][k group] of B in shared memory; four columns of tensor memory per tile,
+// those of A first, then B's row groups side by side.  aoff, boff: 16-byte steps from the first stage.
 template <int GROUP, int NG>
-__device__ __forceinline__ void issue_scales(uint32_t cols, const Desc& xs, const Desc& ws, uint32_t off, int steps) {
+__device__ __forceinline__ void issue_scales(uint32_t cols, const Desc& as, uint32_t aoff, const Desc& bs, uint32_t boff, int steps) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     if (2 * k >= steps) break;
-    scales_to_tmem<GROUP>(cols + 4 * k, xs.at(off + 32 * k));
+    scales_to_tmem<GROUP>(cols + 4 * k, as.at(aoff + 32 * k));
 #pragma unroll
-    for (int g = 0; g < NG; ++g) scales_to_tmem<GROUP>(cols + 8 + (k * NG + g) * 4, ws.at(off + (2 * g + k) * 32));
+    for (int g = 0; g < NG; ++g) scales_to_tmem<GROUP>(cols + 8 + (k * NG + g) * 4, bs.at(boff + (2 * g + k) * 32));
   }
 }
-// The products of one stage.  sb0: columns from the first of W's scales to the tile's own first row.
+// The products of one stage.  sb0: columns from the first of B's scales to the tile's own first row.
 template <int GROUP, int NG>
-__device__ __forceinline__ void issue_products(uint32_t d, const Desc& xc, const Desc& wc, uint32_t off, uint32_t cols, int sb0, uint32_t idesc, int steps, bool first) {
+__device__ __forceinline__ void issue_products(uint32_t d, const Desc& ac, uint32_t aoff, const Desc& bc, uint32_t boff, uint32_t cols, int sb0, uint32_t idesc, int steps, bool first) {
 #pragma unroll
   for (int ks = 0; ks < 4; ++ks) {
     if (ks >= steps) break;
-    mx4_mma<GROUP>(d, xc.at(off + ks * 2), wc.at(off + ks * 2), idesc_half(idesc, ks & 1), cols + 4 * (ks >> 1), cols + 8 + (ks >> 1) * NG * 4 + sb0,
+    mx4_mma<GROUP>(d, ac.at(aoff + ks * 2), bc.at(boff + ks * 2), idesc_half(idesc, ks & 1), cols + 4 * (ks >> 1), cols + 8 + (ks >> 1) * NG * 4 + sb0,
                    first && ks == 0 ? 0u : 1u);
   }
 }

@@ -11,9 +11,12 @@
 // nothing from them.  The sums of an output's digits, each in fp32, are added from the smallest up.  The order of all sums depends on N
 // and K alone: a row has the same bits in every call.
 //
-// mx4_digits_kernel writes the digits into the workspace, a block of 256 rows for each pass over W.  mx4_rows_kernel multiplies: 128 rows of W are the M side, up to
-// 256 digit rows the N side; persistent over W, or one tile per cluster of CTAs that share K where there are few tiles.  The first
-// stages of W are asked for while the digits are still being made.
+// mx4_rows_kernel: 128 rows of W are the M side, up to 256 digit rows the N side; persistent over W, or one tile per cluster of CTAs that
+// share K where there are few tiles.  With few elements of X for a CTA it makes their digits itself, into the tiles that the
+// tensor cores read, while the first stages of W arrive: one launch.  Otherwise mx4_digits_kernel writes them into the workspace, a
+// block of 256 rows for each pass over W, from where they come with every stage, and the first stages of W are asked for while it runs.
+// The line between the two is at 2,048 elements: 1 x 2,048 x 12,352 takes 6.1 us this way and 7.9 that way, 1 x 4,096 x 2,048 (eight CTAs
+// to a row) 6.5 and 7.2; 2 x 2,048 x 131,072 29.3 and 29.0, 4 x 2,048 x 12,352 11.5 and 8.4, since every CTA makes all digits.
 #include <cooperative_groups.h>
 #include "mx4_mma.cuh"
 
@@ -25,17 +28,49 @@ CR_DEFINE_STATUS_WORD(mx4_rows)
 
 constexpr int kDigitsMost = 12, kPassRows = 256;                 // digit rows of a pass over W
 __host__ __device__ constexpr int digits_of(int dtype) { return dtype == CR_ROW_F32 ? 12 : 10; }
-constexpr int kNThreads = 192;                                   // producer, issuer, four epilogue warps
+constexpr int kStream = -1;                                      // digits from the workspace, instead of from rows of a type
+// producer, issuer, four epilogue warps; eight where they make digits before
+__host__ __device__ constexpr int rows_threads(int from) { return from == kStream ? 192 : 320; }
+constexpr int kOwnElements = 2048;                               // elements of X that a CTA turns into digits itself
 constexpr int kNMaxStages = 8;
 constexpr size_t kNRing = 212992;
-constexpr size_t kNSmem = kNRing + (2 * kNMaxStages + 4) * 8 + 16;
+constexpr size_t kNSmem = kNRing + (2 * kNMaxStages + 5) * 8 + 16;
 
 // ---- digits ----------------------------------------------------------------------------------------------------------
-// A thread takes eight elements of a block.
+// The digits of eight elements of a block, whose other elements are with three neighbouring threads (`quad`: the four lanes): for each
+// j the word of codes and the scale byte go to `put`.
+template <int D, typename F>
+__device__ __forceinline__ void make_digits(float (&v)[8], unsigned quad, F&& put) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
+  top = max(top, __shfl_xor_sync(quad, top, 1));
+  top = max(top, __shfl_xor_sync(quad, top, 2));
+  const int field = max((int)(top >> 23), 1);                      // 2^(field - 126) is above every element; 255: not finite
+  const float up = __uint_as_float((uint32_t)(field == 255 ? 1 : 255 - field) << 23);
+  f2 x[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) x[k] = mul2(pack2(v[2 * k], v[2 * k + 1]), pack2(up, up));       // below 4
+  const f2 whole = pack2(12582912.f, 12582912.f), back = pack2(-12582912.f, -12582912.f), minus = pack2(-1.f, -1.f), eight = pack2(8.f, 8.f);
+#pragma unroll
+  for (int j = 0; j < D; ++j) {
+    float d[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const f2 n = add2(add2(x[k], whole), back);                  // 1.5 2^23 leaves no room behind the point: the nearest whole number
+      x[k] = mul2(fma2(n, minus, x[k]), eight);
+      const float2 f = unpack2(n);
+      d[2 * k] = f.x;
+      d[2 * k + 1] = f.y;
+    }
+    const int scale = field - 1 - 3 * j;                           // below 0: what is left lies under 2^-127
+    put(j, field == 255 || scale < 0 ? 0u : pack_e2m1(d, 1.f), field == 255 ? 255 : (uint8_t)max(scale, 0));
+  }
+}
+
 template <int TYPE>
 __global__ void __launch_bounds__(128) mx4_digits_kernel(const void* __restrict__ x, long long ld, bool wide, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                          int rows, int inner, int pass_rows) {
-  constexpr int D = digits_of(TYPE);
   // What stands before this kernel on the stream has ended when the kernel behind it is let in: that one reads the weights at once.
   pdl_wait();
   pdl_release();
@@ -45,30 +80,12 @@ __global__ void __launch_bounds__(128) mx4_digits_kernel(const void* __restrict_
   const int row = (int)(u / per_row), i = (int)(u - (long long)row * per_row);
   float v[8];
   load_row8<TYPE>(x, (size_t)row * ld + (size_t)i * 8, wide, v);
-  uint32_t top = 0;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
-  const unsigned four = 0xfu << (threadIdx.x & 28);
-  top = max(top, __shfl_xor_sync(four, top, 1));
-  top = max(top, __shfl_xor_sync(four, top, 2));
-  const int field = max((int)(top >> 23), 1);                      // 2^(field - 126) is above every element; 255: not finite
-  const float up = __uint_as_float((uint32_t)(field == 255 ? 1 : 255 - field) << 23);
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] *= up;                          // below 4
-  const int at = row / pass_rows * kPassRows + row % pass_rows * D;
+  const int at = row / pass_rows * kPassRows + row % pass_rows * digits_of(TYPE);
   uint32_t* to = reinterpret_cast<uint32_t*>(codes) + (size_t)at * per_row + i;
-#pragma unroll
-  for (int j = 0; j < D; ++j) {
-    const int scale = field - 1 - 3 * j;                           // below 0: what is left lies under 2^-127
-    float d[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      d[k] = rintf(v[k]);
-      v[k] = (v[k] - d[k]) * 8.f;
-    }
-    to[(size_t)j * per_row] = field == 255 || scale < 0 ? 0u : pack_e2m1(d, 1.f);
-    if ((threadIdx.x & 3) == 0) scales[mx4_scale_at(at + j, i >> 2, groups)] = field == 255 ? 255 : (uint8_t)max(scale, 0);
-  }
+  make_digits<digits_of(TYPE)>(v, 0xfu << (threadIdx.x & 28), [&](int j, uint32_t word, uint8_t scale) {
+    to[(size_t)j * per_row] = word;
+    if ((threadIdx.x & 3) == 0) scales[mx4_scale_at(at + j, i >> 2, groups)] = scale;
+  });
 }
 
 // ---- product ----------------------------------------------------------------------------------------------------------------
@@ -76,28 +93,37 @@ struct RowsShape {
   int splits, tiles, passes, pass_rows;                            // CTAs that share K; tiles of W; passes over W, rows of X in each
   int digits, cols;                                                // digits of an element; digit rows of a pass, a multiple of 8
   int stages, stage;                                               // the ring and its stages' bytes
+  const void* x;                                                   // rows whose digits the CTAs make, their pitch, and whether they come 16 bytes at a time
+  long long ld;
+  int wide;
 };
 
-__global__ void __launch_bounds__(kNThreads, 1)
+template <int FROM>
+__global__ void __launch_bounds__(rows_threads(FROM), 1)
 mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ RowsShape S, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                 const __grid_constant__ CUtensorMap wsmap, const __grid_constant__ CUtensorMap xsmap) {
+  constexpr bool OWN = FROM != kStream;
   extern __shared__ __align__(1024) unsigned char sm[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kNRing);
-  uint64_t *full = bars, *empty = bars + kNMaxStages, *accFull = bars + 2 * kNMaxStages, *accEmpty = bars + 2 * kNMaxStages + 2;
-  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 2 * kNMaxStages + 4);
+  uint64_t *full = bars, *empty = bars + kNMaxStages, *accFull = bars + 2 * kNMaxStages, *accEmpty = bars + 2 * kNMaxStages + 2, *ready = bars + 2 * kNMaxStages + 4;
+  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 2 * kNMaxStages + 5);
   volatile int& dead = *reinterpret_cast<volatile int*>(&tmem_slot + 1);
   const int t = threadIdx.x, w = t >> 5, l = t & 31;
   const int split = blockIdx.x % S.splits, first = blockIdx.x / S.splits, step = gridDim.x / S.splits, units = S.tiles * S.passes;
   const int kb_all = (P.K + kXK - 1) / kXK, kb0 = kb_all * split / S.splits, kb_n = kb_all * (split + 1) / S.splits - kb0;
-  const int ST = S.stages, two = S.cols > 128;
+  const int ST = S.stages, two = !OWN && S.cols > 128;
   const int accs = two ? 1 : 2, acc_cols = (S.cols + 31) / 32 * 32, scale_cols = two ? 24 : 16;
+  // The CTA's own digits behind the ring: codes of every stage of K, then their scales.
+  unsigned char *own_codes = sm + ST * S.stage, *own_scales = own_codes + kb_n * S.cols * (kXK / 2);
   if (t == 0) {
     for (int i = 0; i < ST; ++i) { umma::mbar_init(&full[i], 1); umma::mbar_init(&empty[i], 1); }
     for (int i = 0; i < 2; ++i) { umma::mbar_init(&accFull[i], 1); umma::mbar_init(&accEmpty[i], 4); }
+    umma::mbar_init(ready, 8);                                        // the warps that make digits
     umma::mbar_fence_init();
     dead = (umma::smem_u32(sm) & 1023u) != 0;                        // the swizzled tiles need 1 KB boundaries
     if (dead) g_mx4_rows_status = 1;
-    prefetch_map(&wmap); prefetch_map(&xmap); prefetch_map(&wsmap); prefetch_map(&xsmap);
+    prefetch_map(&wmap); prefetch_map(&wsmap);
+    if constexpr (!OWN) { prefetch_map(&xmap); prefetch_map(&xsmap); }
   }
   if (w == 1) umma::tmem_alloc(&tmem_slot, 512);
   umma::fence_before_sync();
@@ -110,7 +136,7 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
     if (gave_up) return;
     if (!umma::mbar_wait_timed(bar, parity, &dead)) { gave_up = true; dead = 1; g_mx4_rows_status = 1; }
   };
-  // A unit is a tile of W and a pass; the passes of a tile follow one another.  Stage: codes of W, scales of W, codes of X, scales of X.
+  // A unit is a tile of W and a pass; the passes of a tile follow one another.  Stage: codes of W, scales of W; scales and codes of X.
   if (w == 0) {
     if (l == 0) {
       // Where a stage comes from and goes to, moved on without a division per stage: they set the pace of the copies otherwise.
@@ -137,23 +163,27 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
         load_box_2d(st, &xsmap, (kb0 + c.kb) * 256, c.pass * (kPassRows / 128), &full[c.s]);
       };
       Cursor cw = begin(), cx = cw;
+      if constexpr (OWN) pdl_wait();                                   // the kernel ahead is the caller's: it may be writing the weights
       for (int i = 0; i < ST && cw.left > 0; ++i) { load_w(cw); advance(cw); }
-      pdl_wait();
-      for (int i = 0; i < ST && cx.left > 0; ++i) { load_x(cx); advance(cx); }
+      if constexpr (!OWN) {
+        pdl_wait();
+        for (int i = 0; i < ST && cx.left > 0; ++i) { load_x(cx); advance(cx); }
+      }
       while (cw.left > 0) {
         wait(&empty[cw.s], cw.phase ^ 1);
         if (gave_up) break;
         load_w(cw);
-        load_x(cw);
+        if constexpr (!OWN) load_x(cw);
         advance(cw);
       }
     }
   } else if (w == 1) {
     const bool one = elect_one();
-    const Desc wc(tma::desc_sw128(sm, 16, 1024)), xc(tma::desc_sw128(sm + kXTile + kXScale * (2 + two), 16, 1024));
-    const Desc ws(umma::smem_desc(sm + kXTile, 0, 128)), xs(umma::smem_desc(sm + kXTile + kXScale, 0, 128));
+    const Desc wc(tma::desc_sw128(sm, 16, 1024)), xc(tma::desc_sw128(OWN ? own_codes : sm + kXTile + kXScale * (2 + two), 16, 1024));
+    const Desc ws(umma::smem_desc(sm + kXTile, 0, 128)), xs(umma::smem_desc(OWN ? own_scales : sm + kXTile + kXScale, 0, 128));
     const uint32_t idesc = idesc_mx4(kXM, S.cols), scales = tm + accs * acc_cols;
     int s = 0, phase = 0, local = 0;
+    if constexpr (OWN) wait(ready, 0);
     for (int u = first; u < units && !gave_up; u += step, ++local) {
       const int a = two ? 0 : local & 1, use = two ? local : local >> 1;
       if (use >= 1) wait(&accEmpty[a], (use - 1) & 1);
@@ -162,14 +192,15 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
         if (gave_up) break;
         umma::fence_after_sync();
         const uint32_t off = s * (S.stage / 16), cols = scales + s * scale_cols;
+        const uint32_t xoff = OWN ? kb * (S.cols * (kXK / 2) / 16) : off, xsoff = OWN ? kb * (kXScale / 16) : off;
         const int steps = P.K / 64 - (kb0 + kb) * 4;
         if (one) {
           if (two) {
-            issue_scales<1, 2>(cols, ws, xs, off, steps);
-            issue_products<1, 2>(tm + a * acc_cols, wc, xc, off, cols, 0, idesc, steps, kb == 0);
+            issue_scales<1, 2>(cols, ws, off, xs, xsoff, steps);
+            issue_products<1, 2>(tm + a * acc_cols, wc, off, xc, xoff, cols, 0, idesc, steps, kb == 0);
           } else {
-            issue_scales<1, 1>(cols, ws, xs, off, steps);
-            issue_products<1, 1>(tm + a * acc_cols, wc, xc, off, cols, 0, idesc, steps, kb == 0);
+            issue_scales<1, 1>(cols, ws, off, xs, xsoff, steps);
+            issue_products<1, 1>(tm + a * acc_cols, wc, off, xc, xoff, cols, 0, idesc, steps, kb == 0);
           }
           umma::commit(&empty[s]);
           if (kb == kb_n - 1) umma::commit(&accFull[a]);
@@ -178,9 +209,28 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
       }
     }
   } else {
+    if constexpr (OWN) {
+      // Eight elements a thread, in the places that a 128-byte-swizzled copy would give them: the 16-byte chunk of a row changes
+      // places with its number xor the row's.
+      pdl_wait();
+      const int D = digits_of(FROM), eights = kb_n * (kXK / 8), k0 = kb0 * kXK;
+      for (int i = t - 64; i < S.pass_rows * eights; i += 256) {
+        const int r = i / eights, e = i - r * eights, kb = e / 32, word = e % 32, b = word / 4;     // b: block of the stage
+        float v[8] = {};
+        if (k0 + e * 8 < P.K) load_row8<FROM>(S.x, (size_t)r * S.ld + k0 + e * 8, S.wide, v);
+        make_digits<digits_of(FROM)>(v, 0xfu << (t & 28), [&](int j, uint32_t codes, uint8_t scale) {
+          const int row = r * D + j;
+          *reinterpret_cast<uint32_t*>(own_codes + kb * S.cols * (kXK / 2) + row * 128 + ((b ^ (row & 7)) << 4) + word % 4 * 4) = codes;
+          if ((t & 3) == 0) own_scales[kb * kXScale + b / 4 * 512 + row % 32 * 16 + row / 32 * 4 + b % 4] = scale;
+        });
+      }
+      umma::fence_async_smem();
+      __syncwarp();
+      if (l == 0) umma::mbar_arrive(ready);
+    }
     const int q = w & 3;
     int local = 0;
-    for (int u = first; u < units; u += step, ++local) {
+    for (int u = first; u < units && w < 6; u += step, ++local) {
       const int a = two ? 0 : local & 1, use = two ? local : local >> 1;
       const int n0 = u / S.passes * 128 + 32 * q, r0 = u % S.passes * S.pass_rows, live = min(S.pass_rows, P.R - r0);
       if (l == 0) wait(&accFull[a], use & 1);
@@ -220,7 +270,7 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
   cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();
   const int n0 = first / S.passes * 128, r0 = first % S.passes * S.pass_rows, outs = min(S.pass_rows, P.R - r0) * 128;
-  for (int i = outs * split / S.splits + t; i < outs * (split + 1) / S.splits; i += kNThreads) {
+  for (int i = outs * split / S.splits + t; i < outs * (split + 1) / S.splits; i += rows_threads(FROM)) {
     float y = 0.f;
     for (int k = 0; k < S.splits; ++k) y += *cluster.map_shared_rank(reinterpret_cast<float*>(sm) + i, k);
     const int col = n0 + i % 128;
@@ -241,15 +291,18 @@ static cr_status rows_splits(int N, int K, int* splits) {
   int dev = 0;
   CR_CUDA(cudaGetDevice(&dev));
   if (cr_status st = once_per_device(configured, [dev] {
-        CR_CUDA(cudaFuncSetAttribute(mx4_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kNSmem));
+        CR_CUDA(cudaFuncSetAttribute(mx4_rows_kernel<kStream>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kNSmem));
+        CR_CUDA(cudaFuncSetAttribute(mx4_rows_kernel<CR_ROW_F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kNSmem));
+        CR_CUDA(cudaFuncSetAttribute(mx4_rows_kernel<CR_ROW_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kNSmem));
+        CR_CUDA(cudaFuncSetAttribute(mx4_rows_kernel<CR_ROW_F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kNSmem));
         for (int s = 1; s <= 8; ++s) {
           cudaLaunchConfig_t cfg = {};
-          cfg.gridDim = dim3(s); cfg.blockDim = dim3(kNThreads); cfg.dynamicSmemBytes = kNSmem;
+          cfg.gridDim = dim3(s); cfg.blockDim = dim3(rows_threads(kStream)); cfg.dynamicSmemBytes = kNSmem;
           cudaLaunchAttribute attr[1];
           attr[0].id = cudaLaunchAttributeClusterDimension;
           attr[0].val.clusterDim.x = s; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
           cfg.attrs = attr; cfg.numAttrs = 1;
-          CR_CUDA(cudaOccupancyMaxActiveClusters(&slots[dev & 63][s], mx4_rows_kernel, &cfg));
+          CR_CUDA(cudaOccupancyMaxActiveClusters(&slots[dev & 63][s], mx4_rows_kernel<kStream>, &cfg));
         }
         return CR_OK;
       })) return st;
@@ -257,6 +310,27 @@ static cr_status rows_splits(int N, int K, int* splits) {
   *splits = 1;
   for (int s = 2; s <= 8 && s <= stages; ++s)
     if (tiles <= slots[dev & 63][s]) *splits = s;
+  return CR_OK;
+}
+
+template <int FROM>
+static cr_status rows_launch(const ProjParams& P, const RowsShape& S, const CUtensorMap (&maps)[4], cudaStream_t stream) {
+  const long long units = (long long)S.tiles * S.passes;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(S.splits > 1 ? units * S.splits : (units < sm_count() ? units : sm_count())));
+  cfg.blockDim = dim3(rows_threads(FROM));
+  cfg.dynamicSmemBytes = kNSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int na = 0;
+  if (pdl_enabled()) { attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[na++].val.programmaticStreamSerializationAllowed = 1; }
+  if (S.splits > 1) {
+    attr[na].id = cudaLaunchAttributeClusterDimension;
+    attr[na].val.clusterDim.x = S.splits; attr[na].val.clusterDim.y = 1; attr[na++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = attr; cfg.numAttrs = na;
+  CR_CUDA(cudaLaunchKernelEx(&cfg, mx4_rows_kernel<FROM>, P, S, maps[0], maps[1], maps[2], maps[3]));
+  CR_LAUNCH_CHECK("mx4_rows_kernel");
   return CR_OK;
 }
 
@@ -293,35 +367,30 @@ extern "C" cr_status cr_mx4_rows(const void* x, cr_row_dtype dtype, long long ld
   S.cols = (S.digits * S.pass_rows + 7) / 8 * 8;
   cr_mx4 d{static_cast<uint8_t*>(workspace), nullptr, S.passes * kPassRows, w->inner};
   d.scales = d.codes + cr_mx4_code_bytes(d.rows, d.inner);
-  S.stage = kXTile + S.cols * (kXK / 2) + (S.cols > 128 ? 3 : 2) * kXScale;
-  S.stages = (int)(kNRing / S.stage < kNMaxStages ? kNRing / S.stage : kNMaxStages);
-  CUtensorMap wmap, wsmap, xmap, xsmap;
-  if (cr_status s = map_mx4(&wmap, &wsmap, w, 128, 1)) return s;
-  if (cr_status s = map_mx4(&xmap, &xsmap, &d, S.cols, S.cols > 128 ? 2 : 1)) return s;
+  const int kb_most = ((w->inner + kXK - 1) / kXK + S.splits - 1) / S.splits;
+  const bool own = S.passes == 1 && S.cols <= 128 && (long long)R * kb_most * kXK <= kOwnElements;
+  S.stage = kXTile + kXScale + (own ? 0 : S.cols * (kXK / 2) + (S.cols > 128 ? 2 : 1) * kXScale);
+  const size_t room = kNRing - (own ? (size_t)kb_most * (S.cols * (kXK / 2) + kXScale) : 0);
+  S.stages = (int)(room / S.stage < kNMaxStages ? room / S.stage : kNMaxStages);
+  S.x = x;
+  S.ld = ld;
+  S.wide = wide_rows(x, dtype, ld);
+  CUtensorMap maps[4];                                               // W, X, scales of W, scales of X
+  if (cr_status s = map_mx4(&maps[0], &maps[2], w, 128, 1)) return s;
   cudaStream_t stream = (cudaStream_t)stream_;
   use_stream(stream);
+  if (own) {
+    maps[1] = maps[0];                                               // not used
+    maps[3] = maps[2];
+    return by_dtype(dtype, [&](auto type) { return rows_launch<decltype(type)::value>(P, S, maps, stream); });
+  }
+  if (cr_status s = map_mx4(&maps[1], &maps[3], &d, S.cols, S.cols > 128 ? 2 : 1)) return s;
   if (cr_status s = by_dtype(dtype, [&](auto type) -> cr_status {
         const long long threads = (long long)R * (w->inner / 8);
-        CR_CUDA(launch_pdl(mx4_digits_kernel<decltype(type)::value>, dim3((unsigned)((threads + 127) / 128)), dim3(128), 0, stream, x, ld, wide_rows(x, dtype, ld),
-                           d.codes, d.scales, R, w->inner, S.pass_rows));
+        CR_CUDA(launch_pdl(mx4_digits_kernel<decltype(type)::value>, dim3((unsigned)((threads + 127) / 128)), dim3(128), 0, stream, x, ld, (bool)S.wide, d.codes, d.scales,
+                           R, w->inner, S.pass_rows));
         CR_LAUNCH_CHECK("mx4_digits_kernel");
         return CR_OK;
       })) return s;
-  const long long units = (long long)S.tiles * S.passes;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(S.splits > 1 ? units * S.splits : (units < sm_count() ? units : sm_count())));
-  cfg.blockDim = dim3(kNThreads);
-  cfg.dynamicSmemBytes = kNSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  int na = 0;
-  if (pdl_enabled()) { attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[na++].val.programmaticStreamSerializationAllowed = 1; }
-  if (S.splits > 1) {
-    attr[na].id = cudaLaunchAttributeClusterDimension;
-    attr[na].val.clusterDim.x = S.splits; attr[na].val.clusterDim.y = 1; attr[na++].val.clusterDim.z = 1;
-  }
-  cfg.attrs = attr; cfg.numAttrs = na;
-  CR_CUDA(cudaLaunchKernelEx(&cfg, mx4_rows_kernel, P, S, wmap, xmap, wsmap, xsmap));
-  CR_LAUNCH_CHECK("mx4_rows_kernel");
-  return CR_OK;
+  return rows_launch<kStream>(P, S, maps, stream);
 }

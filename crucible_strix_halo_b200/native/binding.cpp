@@ -323,10 +323,10 @@ F* present(F* f) {
   return f;
 }
 // A tensor on the current device.
-const at::Tensor& here(PyObject* o, const char* what) {
+const at::Tensor& here(PyObject* o, const char* what, int device = c10::cuda::current_device()) {
   const at::Tensor& t = tensor(o);
   if (!t.is_cuda()) refuse(PyExc_ValueError, "%s must be a CUDA tensor", what);
-  if (t.get_device() != c10::cuda::current_device()) refuse(PyExc_ValueError, "%s is on another device than the current one", what);
+  if (t.get_device() != device) refuse(PyExc_ValueError, "%s is on another device than the current one", what);
   return t;
 }
 cr_row_dtype row_type(const at::Tensor& t, const char* what) {
@@ -351,8 +351,8 @@ int count(int64_t n, const char* what) {
 }
 // `n` elements of a type side by side.
 template <typename T>
-T* flat(PyObject* o, at::ScalarType type, int64_t n, const char* what) {
-  const at::Tensor& t = here(o, what);
+T* flat(PyObject* o, at::ScalarType type, int64_t n, const char* what, int device = c10::cuda::current_device()) {
+  const at::Tensor& t = here(o, what, device);
   if (t.scalar_type() != type) refuse(PyExc_TypeError, "%s has the wrong element type", what);
   if (!t.is_contiguous() || t.numel() < n) refuse(PyExc_ValueError, "%s must be contiguous and long enough", what);
   return static_cast<T*>(t.data_ptr());
@@ -492,26 +492,27 @@ PyObject* logits_choose(PyObject*, PyObject* args) { // (spans, outs or None) ->
     const Py_ssize_t n = PySequence_Fast_GET_SIZE(list.p);
     std::vector<cr_logits_args> a(n);
     Ref outs(PyList_New(n));
+    const int dev = c10::cuda::current_device();
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject* sp = PySequence_Fast_GET_ITEM(list.p, i);
-      const at::Tensor& l = here(item(sp, s_logits), "logits");
+      const at::Tensor& l = here(item(sp, s_logits), "logits", dev);
       a[i] = cr_logits_args{};
       a[i].dtype = row_type(l, "logits");
       a[i].ld = pitch(l, "logits");
       a[i].logits = l.data_ptr();
       const int R = a[i].R = count(l.size(0), "logits"), V = a[i].V = count(l.size(1), "logits");
       if (PyObject* o = item_or_none(sp, s_out)) {
-        const at::Tensor& t = here(o, "out");
+        const at::Tensor& t = here(o, "out", dev);
         if (t.scalar_type() != at::kFloat) refuse(PyExc_TypeError, "%s must be float32", "out");
         a[i].out_ld = pitch(t, "out");
         if (t.size(0) != R || t.size(1) != V) refuse(PyExc_ValueError, "%s has another shape than the logits", "out");
         a[i].out = static_cast<float*>(t.data_ptr());
       }
-      if (PyObject* o = item_or_none(sp, s_counts)) a[i].counts = flat<int>(o, at::kInt, V, "counts");
-      if (PyObject* o = item_or_none(sp, s_drafts)) a[i].drafts = flat<int>(o, at::kInt, R - 1, "drafts");
-      if (PyObject* o = item_or_none(sp, s_bias)) a[i].bias = flat<float>(o, at::kFloat, V, "bias");
+      if (PyObject* o = item_or_none(sp, s_counts)) a[i].counts = flat<int>(o, at::kInt, V, "counts", dev);
+      if (PyObject* o = item_or_none(sp, s_drafts)) a[i].drafts = flat<int>(o, at::kInt, R - 1, "drafts", dev);
+      if (PyObject* o = item_or_none(sp, s_bias)) a[i].bias = flat<float>(o, at::kFloat, V, "bias", dev);
       if (PyObject* o = item_or_none(sp, s_mask)) {
-        const at::Tensor& t = here(o, "mask");
+        const at::Tensor& t = here(o, "mask", dev);
         const int64_t words = ((int64_t)V + 31) / 32;
         if (t.scalar_type() != at::kInt) refuse(PyExc_TypeError, "%s must be int32 words", "mask");
         if (t.dim() == 1 ? t.size(0) < words || (words > 1 && t.stride(0) != 1) : t.dim() != 2 || t.size(0) != R || t.size(1) < words)
@@ -530,7 +531,7 @@ PyObject* logits_choose(PyObject*, PyObject* args) { // (spans, outs or None) ->
         o = wrap(at::empty({R}, at::TensorOptions().dtype(at::kInt).device(l.device())));
       }
       PyList_SET_ITEM(outs.p, i, o);
-      a[i].choice = flat<int>(o, at::kInt, R, "a choice");
+      a[i].choice = flat<int>(o, at::kInt, R, "a choice", dev);
     }
     void* const st = stream();
     check(unlocked([&] { return present(cr_logits_choose)(a.data(), (int)n, st); }));
