@@ -8,13 +8,14 @@ as pending GDN rows that the next pass replays (engine/layers/ops.h:275-293) and
 the accepted positions from the trunk's outputs ("catch-up" rows of an R-row MTP pass).
 
 Everything outside the attention core (embeddings, projections, heads) is the caller's: a `glue` object turns tokens
-and the previous layer's rows into projection rows and output rows into tokens.  This module only orders the calls of
-the C ABI and keeps the ledger; it is host logic, every computation happens in libcrucible_attn.so.
+and the previous layer's rows into projection rows and output rows into tokens.  A stream that is given a Head has its
+tokens chosen by that instead of glue.choose: 4-bit head product, penalties, bias, grammar mask, greedy choice.  This module
+only orders the calls of the C ABI and keeps the ledger; it is host logic, every computation happens in libcrucible_attn.so.
 
 glue protocol:
     gdn_rows(layer, tokens, below)   -> (qkv [R,C], z [R,Hv*128], x [R,hidden])       fp32 cuda tensors
     qsa_rows(tokens, below)          -> (q [R,Hq,512], k [R,Hkv*256], v [R,Hkv*256], idx [R,640])
-    choose(out_rows)                 -> list of R token ids (the target's choice after each row)
+    choose(out_rows)                 -> list of R token ids (the target's choice after each row; not asked of a stream with a Head)
     mtp_rows(tokens, stacks)         -> (q, k, v, idx) of the draft layer for rows (token p+1, stack of position p)
     draft(mtp_out_row, position)     -> one token id
 """
@@ -23,13 +24,51 @@ import torch
 from . import capi, layers
 
 
+class Head:
+    """The head of one stream and its sampler's greedy part: output rows [R, inner] -> tokens.
+
+    w: layers.Mx4 [vocabulary, inner].  repetition, frequency, presence, bias [vocabulary]: as in layers.logits_choose, over all
+    tokens of the stream, prompt included.  allowed: called with the stream's tokens and the drafts of a pass, gives the grammar's
+    words for its 1 + len(drafts) rows (int32, [rows, ceil(vocabulary / 32)] or one row for all), or None where everything is
+    allowed."""
+
+    def __init__(self, w, repetition=1.0, frequency=0.0, presence=0.0, bias=None, allowed=None, rows=capi.MAX_STEP_ROWS):
+        self.w, self.bias, self.allowed = w, bias, allowed
+        self.penalties = dict(repetition=repetition, frequency=frequency, presence=presence)
+        device = w.codes.device
+        self.logits = torch.empty(rows, w.rows, device=device)
+        self.choice = torch.empty(rows, device=device, dtype=torch.int32)
+        self.counts = torch.zeros(w.rows, device=device, dtype=torch.int32)
+
+    def accept(self, tokens):
+        """Tokens that the stream has taken in: from now on they count."""
+        layers.token_count(self.counts, torch.tensor(tokens, device=self.counts.device, dtype=torch.int32))
+
+    def choose(self, out, tokens, drafts=()):
+        """The target's choice after each row of `out`, of which the rows behind the first belong to `drafts`."""
+        R = len(drafts) + 1
+        logits, choice = self.logits[:R], self.choice[:R]
+        layers.mx4_rows(out, self.w, [logits])
+        span = dict(logits=logits, counts=self.counts, bias=self.bias, mask=self.allowed(tokens, drafts) if self.allowed else None, **self.penalties)
+        if drafts:
+            span["drafts"] = torch.tensor(drafts, device=choice.device, dtype=torch.int32)
+        ids = layers.logits_choose([span], [choice])[0].tolist()
+        # Behind a draft that the choice before it refused, a row may have no allowed token: nobody takes it.
+        for r, i in enumerate(ids):
+            if i < 0:
+                raise ValueError("the grammar allows no token after row %d" % r)
+            if r < len(drafts) and drafts[r] != i:
+                break
+        return ids
+
+
 class SpecStream:
     """One request: trunk sessions (GDN layers, then one QSA layer), the draft layer's QSA session, token history and
     the ledger of pending rows."""
 
-    def __init__(self, g, gdn_weights, qsa_weights, mtp_weights, glue, ctx, mtp_rows=0, span=9):
+    def __init__(self, g, gdn_weights, qsa_weights, mtp_weights, glue, ctx, mtp_rows=0, span=9, head=None):
         assert 2 <= span <= capi.MAX_STEP_ROWS
-        self.g, self.glue, self.span = g, glue, span
+        self.g, self.glue, self.span, self.head = g, glue, span, head
         self.gw, self.qw, self.mw = gdn_weights, qsa_weights, mtp_weights
         self.gs = [layers.GdnSession(g, pend_rows=16 if span > 8 else 8) for _ in gdn_weights]
         self.qs = layers.QsaSession(g, ctx, max_rows=capi.MAX_STEP_ROWS)
@@ -60,7 +99,15 @@ class SpecStream:
                 out = self._trunk([self.tokens[-1]], len(self.tokens) - 1, self.replay, 1)
                 self.replay = 0
                 self.stacks = out if self.stacks is None else torch.cat([self.stacks, out])
-            self.tokens.append(int(t))
+            self._take([int(t)])
+
+    def _take(self, tokens):
+        self.tokens += tokens
+        if self.head:
+            self.head.accept(tokens)
+
+    def _choose(self, out, drafts=()):
+        return self.head.choose(out, self.tokens, drafts) if self.head else self.glue.choose(out)
 
     # ---- draft layer -----------------------------------------------------------------------------------------
     def _mtp(self, tokens, stacks, mpos):
@@ -98,14 +145,14 @@ class SpecStream:
         drafts = self._draft(depth)
         rows = [self.tokens[-1]] + drafts
         out = self._trunk(rows, L - 1, self.replay, 1)             # 1 certain row + the drafts, only the first is committed
-        preds = self.glue.choose(out)
+        preds = self._choose(out, drafts)
         n = 0
         while n < depth and drafts[n] == preds[n]:
             n += 1
         self.replay = n                                            # the accepted rows wait in the pending buffers
         self.accepted.append(n)
         emitted = drafts[:n] + [preds[n]]
-        self.tokens += emitted
+        self._take(emitted)
         self.stacks = out[:n + 1] if self.stacks is None or len(self.stacks) == 0 else torch.cat([self.stacks, out[:n + 1]])
         return emitted
 
@@ -114,7 +161,7 @@ class SpecStream:
         out = self._trunk([self.tokens[-1]], len(self.tokens) - 1, self.replay, 1)
         self.replay = 0
         self.stacks = out if self.stacks is None or len(self.stacks) == 0 else torch.cat([self.stacks, out])
-        self.tokens.append(self.glue.choose(out)[0])
+        self._take([self._choose(out)[0]])
         return self.tokens[-1]
 
     def flush(self):
