@@ -222,7 +222,7 @@ extern "C" cr_status cr_token_count(const int* tokens, int n, int delta, int* co
   if (n == 0) return CR_OK;
   cudaStream_t stream = (cudaStream_t)stream_;
   use_stream(stream);
-  const int blocks = (n + 255) / 256;
+  const int blocks = n / 256 + 1;
   CR_CUDA(launch_pdl(token_count_kernel, dim3(blocks < 1024 ? blocks : 1024), dim3(256), 0, stream, tokens, n, delta, counts, V));
   CR_LAUNCH_CHECK("token_count_kernel");
   return CR_OK;

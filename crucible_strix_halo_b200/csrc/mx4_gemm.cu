@@ -114,16 +114,16 @@ mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant
     if (!umma::mbar_wait_timed(bar, parity, &dead)) { gave_up = true; dead = 1; g_mx4_gemm_status = 1; }
   };
 
+  int issued = 0;
   if (w == 0) {
     // ---------------------------------------------------------------- producer (each CTA its own rows of X and of W, all of W's scales)
     if (l == 0) {
-      int it = 0;
+      int s = 0, phase = 1;
       for (int i = pair; i < tiles && !gave_up; i += pairs) {
         int m0, n0;
         tile_at(i, m0, n0);
-        for (int kb = 0; kb < kb_n; ++kb, ++it) {
-          const int s = it % kQStages;
-          if (it >= kQStages) wait(&empty[s], ((it - kQStages) / kQStages) & 1);
+        for (int kb = 0; kb < kb_n; ++kb, ++issued) {
+          if (issued >= kQStages) wait(&empty[s], phase);
           if (gave_up) break;
           unsigned char* st = sm + s * kQStageBytes;
           if (rank == 0) umma::mbar_expect_tx(&full[s], 2 * kQStageBytes);
@@ -132,6 +132,7 @@ mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant
           pair_load_box_2d(st + kXTile, &wmap, kb * (kXK / 2), n0 + 128 * (int)rank, bar);
           pair_load_box_2d(st + 2 * kXTile, &xsmap, kb * 256, m0 / 128 + (int)rank, bar);
           pair_load_box_2d(st + 2 * kXTile + kXScale, &wsmap, kb * 256, n0 / 128, bar);
+          if (++s == kQStages) { s = 0; phase ^= 1; }
         }
       }
     }
@@ -189,6 +190,7 @@ mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant
       }
     }
   }
+  if (dead && rank == 0 && w == 0 && l == 0) drain_copies(full, issued, kQStages);     // both CTAs' copies complete on the leader's barriers
   umma::fence_before_sync();
   __syncwarp();
   cluster.sync();                                                          // neither CTA leaves while the other may still use its memory
@@ -243,11 +245,11 @@ mx4_gemm_split_kernel(const __grid_constant__ ProjParams P, const __grid_constan
     if (gave_up) return;
     if (!umma::mbar_wait_timed(bar, parity, &dead)) { gave_up = true; dead = 1; g_mx4_gemm_status = 1; }
   };
+  int issued = 0;
   if (w == 0) {
     if (l == 0) {
-      for (int it = 0; it < kb_n; ++it) {
-        const int s = it % ST;
-        if (it >= ST) wait(&empty[s], (it / ST - 1) & 1);
+      for (int it = 0, s = 0, phase = 1; it < kb_n; ++it, ++issued) {
+        if (it >= ST) wait(&empty[s], phase);
         if (gave_up) break;
         unsigned char* st = sm + s * stage;
         umma::mbar_expect_tx(&full[s], stage);
@@ -255,6 +257,7 @@ mx4_gemm_split_kernel(const __grid_constant__ ProjParams P, const __grid_constan
         load_box_2d(st, &xmap, (kb0 + it) * (kXK / 2), m0, &full[s]);
         load_box_2d(st + xbytes + TN * (kXK / 2), &xsmap, (kb0 + it) * 256, m0 / 128, &full[s]);
         load_box_2d(st + xbytes + TN * (kXK / 2) + kXScale, &wsmap, (kb0 + it) * 256, n0 / 128, &full[s]);
+        if (++s == ST) { s = 0; phase ^= 1; }
       }
     }
   } else if (w == 1) {
@@ -298,6 +301,7 @@ mx4_gemm_split_kernel(const __grid_constant__ ProjParams P, const __grid_constan
   }
   umma::fence_before_sync();
   __syncthreads();
+  if (dead && w == 0 && l == 0) drain_copies(full, issued, ST);
   if (w == 1) umma::tmem_dealloc(tm, 512);
   if (splits == 1) return;
   // Every CTA of the cluster sums a slice of the rows over all partial tiles, in the order of K.

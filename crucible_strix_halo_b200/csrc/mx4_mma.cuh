@@ -83,6 +83,12 @@ __device__ __forceinline__ void issue_products(uint32_t d, const Desc& ac, uint3
   }
 }
 
+// After a wait has given up, by the thread that issued the copies: no CTA ends before its last copies have landed, for a millisecond
+// each at most.  `issued` stages went into a ring of `ring`.
+__device__ __forceinline__ void drain_copies(uint64_t* full, int issued, int ring) {
+  for (int i = issued > ring ? issued - ring : 0; i < issued; ++i) umma::mbar_wait_timed(&full[i % ring], (i / ring) & 1, nullptr, 1000000);
+}
+
 // Codes as a tensor map of bytes with boxes of box_rows x 128 bytes, 128-byte swizzle; scales as words, a row of the map for a row
 // group, boxes of two tiles by box_groups.  Past the edges the copy engine fills in zeros.
 inline cr_status map_mx4(CUtensorMap* codes, CUtensorMap* scales, const cr_mx4* m, int box_rows, int box_groups) {

@@ -136,6 +136,7 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
     if (gave_up) return;
     if (!umma::mbar_wait_timed(bar, parity, &dead)) { gave_up = true; dead = 1; g_mx4_rows_status = 1; }
   };
+  int issued = 0;
   // A unit is a tile of W and a pass; the passes of a tile follow one another.  Stage: codes of W, scales of W; scales and codes of X.
   if (w == 0) {
     if (l == 0) {
@@ -176,6 +177,7 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
         if constexpr (!OWN) load_x(cw);
         advance(cw);
       }
+      issued = own * kb_n - cw.left;
     }
   } else if (w == 1) {
     const bool one = elect_one();
@@ -264,6 +266,7 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
   }
   umma::fence_before_sync();
   __syncthreads();
+  if (dead && w == 0 && l == 0) drain_copies(full, issued, ST);
   if (w == 1) umma::tmem_dealloc(tm, 512);
   if (S.splits == 1) return;
   // One unit per cluster: each CTA adds a part of the outputs over all shares of K, in their order.

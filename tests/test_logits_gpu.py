@@ -166,6 +166,16 @@ def test_infinities_and_nans_in_allowed_places():
     assert c[:4] == [1500, 1999, 0, 7]
 
 
+@pytest.mark.parametrize("dtype,bits", [(torch.float32, -1), (torch.float32, -0x400000), (torch.bfloat16, -1), (torch.float16, -1)])
+def test_a_nan_of_either_sign_is_the_largest(dtype, bits):
+    logits = torch.randn(1, 900, device="cuda").to(dtype)
+    view = logits.view(torch.int32 if dtype == torch.float32 else torch.int16)
+    view[0, 500] = bits
+    logits[0, 600] = math.nan
+    logits[0, 700] = math.inf
+    assert check([dict(logits=logits, out=torch.empty(1, 900, device="cuda"))])[0].tolist() == [500]
+
+
 def test_logits_of_the_types_lowest_value():
     V = 3000
     for dtype in TYPES:
@@ -232,6 +242,20 @@ def test_captured_calls_replay_on_new_inputs():
         assert torch.equal(outs[0], want)
         before[want[0].long()] += 1
         assert torch.equal(sp["counts"], before)
+
+
+def test_calls_on_two_streams_do_not_disturb_each_other():
+    L = layers()
+    spans = [span(9, 30000, i, mask="rows") for i in range(2)]
+    want = [L.logits_choose([sp])[0] for sp in spans]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(20):
+        for s, sp in zip(streams, spans):
+            with torch.cuda.stream(s):
+                got.append(L.logits_choose([sp])[0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(c, want[i % 2]) for i, c in enumerate(got))
 
 
 @pytest.mark.parametrize("change,error", [

@@ -378,6 +378,31 @@ def test_calls_on_two_streams_do_not_disturb_each_other():
         assert torch.equal(a, want[i % 2][0]) and torch.equal(b, want[i % 2][1])
 
 
+def test_plain_launches_give_the_same_bits():
+    """Without programmatic dependent launches the same kernels run one after the other."""
+    from crucible_strix_halo_b200 import capi
+    L = layers()
+    K, N = 2560, 4128
+    x, w = torch.randn(60, K, device="cuda").bfloat16(), random_mx4(N, K, 1)
+    xq = random_mx4(300, K, 2)
+
+    def calls():
+        y = [torch.empty(r, N, device="cuda") for r in (1, 9, 60, 300)]
+        L.mx4_rows(x[:1], w, y[:1])
+        L.mx4_rows(x[:9], w, y[1:2])
+        L.mx4_rows(x, w, y[2:3])
+        L.mx4_gemm(xq, w, y[3:])
+        return y + [L.mx4_dequant(L.mx4_quant(x))]
+    want = calls()
+    capi.set_options(pdl=0)
+    try:
+        got = calls()
+    finally:
+        capi.set_options(pdl=1)
+    status()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_a_projection_chain_as_a_prompt_and_as_steps():
     """Prompt rows through quantise, 4-bit input projection and the GDN core; the input projection of the same rows as verify rows
     gives the core's rows of the same numbers."""
