@@ -5,8 +5,11 @@
 // 32, so that rows of any pitch and address are read a line at a time, the next 256 while these are worked on.  Counts and biases
 // come from L2 after the first row.  The division by the repetition penalty is left to the runs that hold a repeated token.  The best
 // token goes from thread to warp to CTA, and the CTAs' are gathered through distributed shared memory: one launch, no scratch.
-// All rows of a span in one cluster, with counts, biases and keys of twelve rows in registers, took 90 us for 8 x 9 rows of 100,352
-// (87 instructions a token, a sixth of the time waiting for them to be fetched).
+// What bounds it: instructions, about 45 a token with everything asked for (8 x 9 rows of 100,352 in bf16 with mask and processed logits
+// 27.5 us, 16 x 13 rows of 131,072 70 us, 3.3 TB/s); latency for one row (5.7 us at 131,071 tokens).  CTAs of 1,024 threads while one wave
+// holds all rows, of 256 otherwise (the second call 82 us with 512).  Taken back: all rows of a span in one cluster, with counts, biases and
+// keys of twelve rows in registers (90 us); one comparison for the eight tokens of a lane with a search behind it (84 us for the
+// second call: in every piece some lane finds a better token); pieces of 128 tokens (94 us).
 #include <cooperative_groups.h>
 #include "mx4.cuh"
 
@@ -210,7 +213,7 @@ extern "C" cr_status cr_logits_choose(const cr_logits_args* spans, int n_spans, 
     for (int i = 0; i < n; ++i) { T.s[i] = spans[i0 + i]; rows = rows > T.s[i].R ? rows : T.s[i].R; }
     const dim3 grid((unsigned)(kChooseCluster * rows), n);
     if (rows * n * kChooseCluster <= sm_count()) CR_CUDA(launch_pdl(logits_choose_kernel<1024>, grid, dim3(1024), 0, stream, T));
-    else CR_CUDA(launch_pdl(logits_choose_kernel<512>, grid, dim3(512), 0, stream, T));
+    else CR_CUDA(launch_pdl(logits_choose_kernel<256>, grid, dim3(256), 0, stream, T));
     CR_LAUNCH_CHECK("logits_choose_kernel");
   }
   return CR_OK;
