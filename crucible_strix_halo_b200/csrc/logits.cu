@@ -3,7 +3,7 @@
 //
 // HBM-bound with many rows, latency-bound with one: a cluster of eight CTAs takes a row, its warps 256 tokens at a time in eight runs of
 // 32, so that rows of any pitch and address are read a line at a time, the next 256 while these are worked on.  Counts and biases
-// come from L2 after the first row.  The division by the repetition penalty is left to the runs that hold a repeated token.  The best
+// come from L2 after the first row.  The division by the repetition penalty is left to the pieces that hold a repeated token.  The best
 // token goes from thread to warp to CTA, and the CTAs' are gathered through distributed shared memory: one launch, no scratch.
 // What bounds it: instructions, about 45 a token with everything asked for (8 x 9 rows of 100,352 in bf16 with mask and processed logits
 // 27.5 us, 16 x 13 rows of 131,072 70 us, 3.3 TB/s); latency for one row (5.7 us at 131,071 tokens).  CTAs of 1,024 threads while one wave

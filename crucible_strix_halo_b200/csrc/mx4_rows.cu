@@ -17,6 +17,11 @@
 // block of 256 rows for each pass over W, from where they come with every stage, and the first stages of W are asked for while it runs.
 // The line between the two is at 2,048 elements: 1 x 2,048 x 12,352 takes 6.1 us this way and 7.9 that way, 1 x 4,096 x 2,048 (eight CTAs
 // to a row) 6.5 and 7.2; 2 x 2,048 x 131,072 29.3 and 29.0, 4 x 2,048 x 12,352 11.5 and 8.4, since every CTA makes all digits.
+//
+// What bounds it: W at 131,072 x 2,048 is 142.6 MB, 21.8 us at the copy bandwidth and 22.6 us for the same copies without products.  One row
+// takes 26.3 us, 9 rows 30.8, 13 rows 32.2 (4.6 TB/s): the launches, the first stage's and the last tile's latency, 4 to 7 us.  The
+// copying thread's divisions had cost 4 us; one accumulator for 11 to 19 rows 13 us, since the epilogue stands between two tiles then.
+// 20 to 25 rows have one (48 to 54 us).  Calls over few weights are latencies: 1 x 64 x 32 3.6 us.
 #include <cooperative_groups.h>
 #include "mx4_mma.cuh"
 
@@ -28,6 +33,7 @@ CR_DEFINE_STATUS_WORD(mx4_rows)
 
 constexpr int kDigitsMost = 12, kPassRows = 256;                 // digit rows of a pass over W
 __host__ __device__ constexpr int digits_of(int dtype) { return dtype == CR_ROW_F32 ? 12 : 10; }
+constexpr int kRowsMost = kPassRows / digits_of(CR_ROW_BF16);    // rows of X of a pass
 constexpr int kStream = -1;                                      // digits from the workspace, instead of from rows of a type
 // producer, issuer, four epilogue warps; eight where they make digits before
 __host__ __device__ constexpr int rows_threads(int from) { return from == kStream ? 192 : 320; }
@@ -92,11 +98,15 @@ __global__ void __launch_bounds__(128) mx4_digits_kernel(const void* __restrict_
 struct RowsShape {
   int splits, tiles, passes, pass_rows;                            // CTAs that share K; tiles of W; passes over W, rows of X in each
   int digits, cols;                                                // digits of an element; digit rows of a pass, a multiple of 8
-  int stages, stage;                                               // the ring and its stages' bytes
+  int stages, stage, accs;                                         // the ring and its stages' bytes; accumulators
   const void* x;                                                   // rows whose digits the CTAs make, their pitch, and whether they come 16 bytes at a time
   long long ld;
   int wide;
 };
+
+// Columns of tensor memory: an accumulator's (read 16 at a time from a row's first digit on) and the scales' of a stage.
+__host__ __device__ inline int acc_columns(int cols) { return (cols + 31) / 32 * 32; }
+__host__ __device__ inline int scale_columns(int cols) { return cols > 128 ? 24 : 16; }
 
 template <int FROM>
 __global__ void __launch_bounds__(rows_threads(FROM), 1)
@@ -112,7 +122,7 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
   const int split = blockIdx.x % S.splits, first = blockIdx.x / S.splits, step = gridDim.x / S.splits, units = S.tiles * S.passes;
   const int kb_all = (P.K + kXK - 1) / kXK, kb0 = kb_all * split / S.splits, kb_n = kb_all * (split + 1) / S.splits - kb0;
   const int ST = S.stages, two = !OWN && S.cols > 128;
-  const int accs = two ? 1 : 2, acc_cols = (S.cols + 31) / 32 * 32, scale_cols = two ? 24 : 16;
+  const int accs = S.accs, acc_cols = acc_columns(S.cols), scale_cols = scale_columns(S.cols);
   // The CTA's own digits behind the ring: codes of every stage of K, then their scales.
   unsigned char *own_codes = sm + ST * S.stage, *own_scales = own_codes + kb_n * S.cols * (kXK / 2);
   if (t == 0) {
@@ -187,7 +197,7 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
     int s = 0, phase = 0, local = 0;
     if constexpr (OWN) wait(ready, 0);
     for (int u = first; u < units && !gave_up; u += step, ++local) {
-      const int a = two ? 0 : local & 1, use = two ? local : local >> 1;
+      const int a = accs == 2 ? local & 1 : 0, use = accs == 2 ? local >> 1 : local;
       if (use >= 1) wait(&accEmpty[a], (use - 1) & 1);
       for (int kb = 0; kb < kb_n; ++kb) {
         wait(&full[s], phase);
@@ -233,7 +243,7 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
     const int q = w & 3;
     int local = 0;
     for (int u = first; u < units && w < 6; u += step, ++local) {
-      const int a = two ? 0 : local & 1, use = two ? local : local >> 1;
+      const int a = accs == 2 ? local & 1 : 0, use = accs == 2 ? local >> 1 : local;
       const int n0 = u / S.passes * 128 + 32 * q, r0 = u % S.passes * S.pass_rows, live = min(S.pass_rows, P.R - r0);
       if (l == 0) wait(&accFull[a], use & 1);
       __syncwarp();
@@ -241,25 +251,29 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
       umma::fence_after_sync();
       int o = 0;
       while (o < P.n_outs - 1 && n0 >= P.col0[o] + P.cols[o]) ++o;     // 32 columns never straddle outputs
-#pragma unroll 1
-      for (int r = 0; r < live; ++r) {
+      float y[kRowsMost];
+#pragma unroll
+      for (int r = 0; r < kRowsMost; ++r) {
+        if (r >= live) break;
         float v[16];
         umma::tmem_ld16(umma::tmem_addr(tm, q, a * acc_cols + r * S.digits), v);     // warp-collective
-        if (r + 1 == live) {
-          umma::fence_before_sync();
-          __syncwarp();
-          if (l == 0) umma::mbar_arrive_relaxed(&accEmpty[a]);
-        }
-        float y = 0.f;
+        y[r] = 0.f;
 #pragma unroll
         for (int j = kDigitsMost - 1; j >= 0; --j)
-          if (j < S.digits) y += v[j];
+          if (j < S.digits) y[r] += v[j];
+      }
+      umma::fence_before_sync();
+      __syncwarp();
+      if (l == 0) umma::mbar_arrive_relaxed(&accEmpty[a]);                  // the next tile's products may come
+#pragma unroll
+      for (int r = 0; r < kRowsMost; ++r) {
+        if (r >= live) break;
         if (S.splits > 1) {
-          reinterpret_cast<float*>(sm)[r * 128 + 32 * q + l] = y;                     // every stage has been read
+          reinterpret_cast<float*>(sm)[r * 128 + 32 * q + l] = y[r];                  // every stage has been read
         } else if (n0 < P.N) {
           const size_t at = (size_t)(r0 + r) * P.ld[o] + (n0 + l - P.col0[o]);
-          if (P.f32[o]) reinterpret_cast<float*>(P.ptr[o])[at] = y;
-          else reinterpret_cast<__nv_bfloat16*>(P.ptr[o])[at] = __float2bfloat16_rn(y);
+          if (P.f32[o]) reinterpret_cast<float*>(P.ptr[o])[at] = y[r];
+          else reinterpret_cast<__nv_bfloat16*>(P.ptr[o])[at] = __float2bfloat16_rn(y[r]);
         }
       }
     }
@@ -374,7 +388,10 @@ extern "C" cr_status cr_mx4_rows(const void* x, cr_row_dtype dtype, long long ld
   const bool own = S.passes == 1 && S.cols <= 128 && (long long)R * kb_most * kXK <= kOwnElements;
   S.stage = kXTile + kXScale + (own ? 0 : S.cols * (kXK / 2) + (S.cols > 128 ? 2 : 1) * kXScale);
   const size_t room = kNRing - (own ? (size_t)kb_most * (S.cols * (kXK / 2) + kXScale) : 0);
-  S.stages = (int)(room / S.stage < kNMaxStages ? room / S.stage : kNMaxStages);
+  // Two accumulators while they leave columns for the scales of four stages: the epilogue of a tile beside the products of the next.
+  S.accs = 2 * acc_columns(S.cols) + 4 * scale_columns(S.cols) <= 512 ? 2 : 1;
+  const int columned = (512 - S.accs * acc_columns(S.cols)) / scale_columns(S.cols), most = columned < kNMaxStages ? columned : kNMaxStages;
+  S.stages = (int)(room / S.stage) < most ? (int)(room / S.stage) : most;
   S.x = x;
   S.ld = ld;
   S.wide = wide_rows(x, dtype, ld);
