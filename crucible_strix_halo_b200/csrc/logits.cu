@@ -1,15 +1,18 @@
 // Penalties, biases and grammar masks on the logits of spans, and the greedy choice (see cr_logits_choose for the formula).
 // Every product, quotient and sum is rounded by itself (no contraction), so that a choice is the definition's own.
 //
-// HBM-bound with many rows, latency-bound with one: a cluster of eight CTAs takes a row, its warps 256 tokens at a time in eight runs of
-// 32, so that rows of any pitch and address are read a line at a time, the next 256 while these are worked on.  Counts and biases
-// come from L2 after the first row.  The division by the repetition penalty is left to the pieces that hold a repeated token.  The best
-// token goes from thread to warp to CTA, and the CTAs' are gathered through distributed shared memory: one launch, no scratch.
-// What bounds it: instructions, about 45 a token with everything asked for (8 x 9 rows of 100,352 in bf16 with mask and processed logits
-// 27.5 us, 16 x 13 rows of 131,072 70 us, 3.3 TB/s); latency for one row (5.7 us at 131,071 tokens).  CTAs of 1,024 threads while one wave
-// holds all rows, of 256 otherwise (the second call 82 us with 512).  Taken back: all rows of a span in one cluster, with counts, biases and
-// keys of twelve rows in registers (90 us); one comparison for the eight tokens of a lane with a search behind it (84 us for the
-// second call: in every piece some lane finds a better token); pieces of 128 tokens (94 us).
+// A cluster of eight CTAs takes a row, its warps 256 tokens at a time: four and four of a lane lie together where the addresses allow
+// it, else a run of 32 after another, so that rows of any pitch and address are read whole lines at a time.  The next 256 logits are
+// asked for while these are worked on.  Counts and biases come from L2 after the first row; a span's drafts stay in a register of a lane
+// each.  The division by the repetition penalty is left to the pieces that hold a repeated token.  The best token goes from thread to warp
+// to CTA, and the CTAs' are gathered through distributed shared memory: one launch, no scratch.
+//
+// What bounds it: with many rows the chain of a piece's loads and some 40 instructions a token (16 x 13 rows of 131,072, fp32, mask and
+// processed logits: 58 us, 4.0 TB/s; 8 x 9 rows of 100,352 in bf16: 26 us); with one row latency (5.7 us at 131,071 tokens).  CTAs of 1,024
+// threads while one wave holds all rows, of 256 otherwise (82 us for the first call with 512).  Drafts read from memory for every piece
+// and runs of 32 alone: 70 us.  Taken back: all rows of a span in one cluster, with counts, biases and keys of twelve rows in registers
+// (8 x 9 rows 90 us); one comparison for the eight tokens of a lane with a search behind it (85 us for 16 x 13: in every piece some lane
+// finds a better token); pieces of 128 tokens (94 us); fewer registers and five CTAs on an SM (8 x 9 rows 25 us, 16 x 13 rows 79 us).
 #include <cooperative_groups.h>
 #include "mx4.cuh"
 
@@ -42,29 +45,51 @@ __device__ __forceinline__ float logit_value(uint32_t u) {
 // What a warp has found: key and index of its lanes' best tokens.
 struct Best { uint32_t key = 0; int at = 0; };
 
-// 256 tokens from v0 on; FULL: all of them below V.
-template <bool FULL>
-__device__ __forceinline__ void choose_piece(const cr_logits_args& a, int r, int v0, float (&x)[8], const uint32_t* mask, float* out, Best& best) {
+// A lane's eight of 256 tokens: one of each run of 32, or (WIDE, where every address allows it) four and four that lie together.
+template <bool WIDE>
+__device__ __forceinline__ int token_of(int k, int l) { return WIDE ? (k >> 2) * 128 + 4 * l + (k & 3) : 32 * k + l; }
+
+// Eight 32-bit values of a lane's tokens from p (the piece's first); FULL: all of them below `left`.
+template <bool FULL, bool WIDE, typename T>
+__device__ __forceinline__ void load_tokens(const T* p, int left, T (&v)[8]) {
+  static_assert(sizeof(T) == 4, "");
   const int l = threadIdx.x & 31;
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int4 u = *reinterpret_cast<const int4*>(p + 128 * j + 4 * l);
+      v[4 * j] = reinterpret_cast<const T&>(u.x); v[4 * j + 1] = reinterpret_cast<const T&>(u.y);
+      v[4 * j + 2] = reinterpret_cast<const T&>(u.z); v[4 * j + 3] = reinterpret_cast<const T&>(u.w);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = FULL || 32 * k + l < left ? p[32 * k + l] : T(0);
+  }
+}
+
+// 256 tokens from v0 on; FULL: all of them below V.
+template <bool FULL, bool WIDE>
+__device__ __forceinline__ void choose_piece(const cr_logits_args& a, int r, int v0, int draft, float (&x)[8], const uint32_t* mask, float* out, Best& best) {
+  const int l = threadIdx.x & 31, left = a.V - v0;
   int n[8];
   bool said = false;
 #pragma unroll
   for (int k = 0; k < 8; ++k) n[k] = 0;
-  if (a.counts) {
-    const int* p = a.counts + v0 + l;
+  if (a.counts) load_tokens<FULL, WIDE>(a.counts + v0, left, n);
+  uint32_t word = 0xffffffffu;                                            // lane k < 8 has the words of tokens 32 k on
+  if (mask && l < 8 && (FULL || 32 * l < left)) word = mask[(v0 >> 5) + l];
+  float add[8];
+  if (a.bias) load_tokens<FULL, WIDE>(a.bias + v0, left, add);
+  // Drafts that lie in the piece: lane j has the j-th of them.
+  for (int j0 = 0;;) {
+    for (uint32_t hits = __ballot_sync(0xffffffffu, (unsigned)(draft - v0) < 256u); hits; hits &= hits - 1) {
+      const int d = __shfl_sync(0xffffffffu, draft, __ffs(hits) - 1) - v0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) n[k] = FULL || v0 + 32 * k + l < a.V ? p[32 * k] : 0;
-  }
-  uint32_t word = 0xffffffffu;                                            // lane k < 8 has the words of run k
-  if (mask && l < 8 && (FULL || v0 + 32 * l < a.V)) word = mask[(v0 >> 5) + l];
-  if (a.drafts)
-    for (int j = 0; j < r; ++j) {
-      const int d = a.drafts[j] - v0;
-      if ((unsigned)d < 256u) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) n[k] += d == 32 * k + l;
-      }
+      for (int k = 0; k < 8; ++k) n[k] += d == token_of<WIDE>(k, l);
     }
+    if ((j0 += 32) >= r || !a.drafts) break;
+    draft = j0 + l < r ? a.drafts[j0 + l] : -1;
+  }
 #pragma unroll
   for (int k = 0; k < 8; ++k) said |= n[k] > 0;
   if (__any_sync(0xffffffffu, said)) {
@@ -76,55 +101,73 @@ __device__ __forceinline__ void choose_piece(const cr_logits_args& a, int r, int
       }
   }
   if (a.bias) {
-    const float* p = a.bias + v0 + l;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = __fadd_rn(x[k], FULL || v0 + 32 * k + l < a.V ? p[32 * k] : 0.f);
+    for (int k = 0; k < 8; ++k) x[k] = __fadd_rn(x[k], add[k]);
   }
   if (mask) {
-    uint32_t mine = 0;                                                    // bit k: token 32 k + l is allowed
+    uint32_t mine = 0;                                                    // bit k: the lane's token k is allowed
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) mine |= (__shfl_sync(0xffffffffu, word, k) >> l & 1) << k;
+      for (int j = 0; j < 2; ++j) mine |= (__shfl_sync(0xffffffffu, word, 4 * j + (l >> 3)) >> (4 * (l & 7)) & 15) << (4 * j);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mine |= (__shfl_sync(0xffffffffu, word, k) >> l & 1) << k;
+    }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const bool allowed = mine >> k & 1;
       const uint32_t o = order_key(x[k]);
       x[k] = allowed ? x[k] : -INFINITY;
-      if (allowed && (FULL || v0 + 32 * k + l < a.V) && o > best.key) { best.key = o; best.at = v0 + 32 * k + l; }
+      if (allowed && (FULL || 32 * k + l < left) && o > best.key) { best.key = o; best.at = v0 + token_of<WIDE>(k, l); }
     }
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const uint32_t o = order_key(x[k]);
-      if ((FULL || v0 + 32 * k + l < a.V) && o > best.key) { best.key = o; best.at = v0 + 32 * k + l; }
+      if ((FULL || 32 * k + l < left) && o > best.key) { best.key = o; best.at = v0 + token_of<WIDE>(k, l); }
     }
   }
   if (out) {
-    float* p = out + v0 + l;
+    float* p = out + v0;
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (FULL || v0 + 32 * k + l < a.V) __stcs(p + 32 * k, x[k]);
+      for (int j = 0; j < 2; ++j) __stcs(reinterpret_cast<float4*>(p + 128 * j + 4 * l), make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (FULL || 32 * k + l < left) __stcs(p + 32 * k + l, x[k]);
+    }
   }
 }
 
 // Row r, the tokens of this warp out of `warps`.  Returns the warp's best: key and complement of the index, so that the larger number
 // is the better token and the lower index among equals; 0 where none is allowed.
-template <int TYPE>
+template <int TYPE, bool WIDE>
 __device__ __forceinline__ uint64_t choose_row(const cr_logits_args& a, int r, int warp, int warps) {
   constexpr int SIZE = TYPE == CR_ROW_F32 ? 4 : 2;
   const int l = threadIdx.x & 31, step = warps * 256;
-  const char* row = static_cast<const char*>(a.logits) + ((size_t)r * a.ld + l) * SIZE;
+  const char* row = static_cast<const char*>(a.logits) + (size_t)r * a.ld * SIZE;
   float* out = a.out ? a.out + (size_t)r * a.out_ld : nullptr;
   const uint32_t* mask = a.mask ? a.mask + (size_t)r * a.mask_ld : nullptr;
+  const int draft = a.drafts && l < r ? a.drafts[l] : -1;
   Best best;
-  uint32_t ahead[8];
+  uint32_t ahead[8];                                                       // of 16-bit logits two to a word where they are loaded so
   auto fetch = [&](int v0) {
     const char* p = row + (size_t)v0 * SIZE;
-    if (v0 + 256 <= a.V) {
+    if (WIDE && v0 + 256 <= a.V) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) ahead[k] = logit_bits<TYPE>(p + 32 * k * SIZE);
+      for (int j = 0; j < 2; ++j) {
+        if constexpr (SIZE == 4) {
+          const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p) + 32 * j + l);
+          ahead[4 * j] = u.x; ahead[4 * j + 1] = u.y; ahead[4 * j + 2] = u.z; ahead[4 * j + 3] = u.w;
+        } else {
+          const uint2 u = __ldcs(reinterpret_cast<const uint2*>(p) + 32 * j + l);
+          ahead[4 * j] = u.x & 0xffffu; ahead[4 * j + 1] = u.x >> 16; ahead[4 * j + 2] = u.y & 0xffffu; ahead[4 * j + 3] = u.y >> 16;
+        }
+      }
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) ahead[k] = v0 + 32 * k + l < a.V ? logit_bits<TYPE>(p + 32 * k * SIZE) : 0;
+      for (int k = 0; k < 8; ++k) ahead[k] = v0 + 32 * k + l < a.V ? logit_bits<TYPE>(p + (32 * k + l) * SIZE) : 0;
     }
   };
   if (warp * 256 < a.V) fetch(warp * 256);
@@ -134,12 +177,19 @@ __device__ __forceinline__ uint64_t choose_row(const cr_logits_args& a, int r, i
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = logit_value<TYPE>(ahead[k]);
     if (v0 + step < a.V) fetch(v0 + step);
-    if (v0 + 256 <= a.V) choose_piece<true>(a, r, v0, x, mask, out, best);
-    else choose_piece<false>(a, r, v0, x, mask, out, best);
+    if (v0 + 256 <= a.V) choose_piece<true, WIDE>(a, r, v0, draft, x, mask, out, best);
+    else choose_piece<false, false>(a, r, v0, draft, x, mask, out, best);
   }
   const uint32_t top = __reduce_max_sync(0xffffffffu, best.key);
   const uint32_t low = __reduce_min_sync(0xffffffffu, best.key == top ? (uint32_t)best.at : 0xffffffffu);
   return top ? (uint64_t)top << 32 | (uint32_t)~low : 0;
+}
+template <int TYPE>
+__device__ __forceinline__ uint64_t choose_row(const cr_logits_args& a, int r, int warp, int warps) {
+  constexpr size_t SIZE = TYPE == CR_ROW_F32 ? 4 : 2;
+  const uintptr_t row = (uintptr_t)a.logits + (size_t)r * a.ld * SIZE, out = (uintptr_t)a.out + (a.out ? (size_t)r * a.out_ld * 4 : 0);
+  const bool wide = ((row & (4 * SIZE - 1)) | (out & 15) | ((uintptr_t)a.counts & 15) | ((uintptr_t)a.bias & 15)) == 0;
+  return wide ? choose_row<TYPE, true>(a, r, warp, warps) : choose_row<TYPE, false>(a, r, warp, warps);
 }
 
 // grid: (8 CTAs x rows, spans).
