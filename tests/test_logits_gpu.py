@@ -205,6 +205,29 @@ def test_rows_at_any_pitch_and_address(offset, pitch, dtype):
     assert (out == 7).all()
 
 
+@pytest.mark.parametrize("what", ["counts", "bias", "out", "logits"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_buffer_off_the_others_alignment(what, dtype):
+    V = 4100
+    sp = span(3, V, 8, dtype, mask="rows")
+    if what in ("counts", "bias"):
+        off = torch.zeros(V + 1, device="cuda", dtype=sp[what].dtype)
+        off[1:] = sp[what]
+        sp[what] = off[1:]
+    else:
+        off = torch.zeros(3 * V + 1, device="cuda", dtype=sp[what].dtype)
+        off[1:] = sp[what].flatten()
+        sp[what] = off[1:].view(3, V)
+    check([sp])
+
+
+def test_more_drafts_than_a_warp_has_lanes():
+    V = 600
+    sp = span(75, V, 9, drafts=False)
+    sp["drafts"] = torch.tensor([5, 255, 256, 599] * 18 + [5, 5], device="cuda", dtype=torch.int32)
+    check([sp])
+
+
 def test_counts_are_kept():
     L = layers()
     V = 1000
