@@ -364,7 +364,8 @@ cr_status cr_proj_gemm(const void* x, const void* w, int R, int K, int N, const 
  * scales  tiles of 128 rows x 4 blocks (512 bytes), all tiles of a row group after one another: block b of row r is byte
  *         (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4 of tile (r / 128) * ceil(inner / 128) + b / 4.  Bytes of the last tiles that
  *         belong to no row or block are neither written nor matter.
- * Both 16-byte aligned.  rows >= 1, inner a multiple of 64, both below 2^24. */
+ * Both 16-byte aligned.  rows >= 1, inner a multiple of 64, both below 2^24 (and rows * ceil(inner / 256) below 2^31 in the two
+ * conversions). */
 typedef struct {
   uint8_t* codes;
   uint8_t* scales;
@@ -391,11 +392,12 @@ cr_status cr_mx4_dequant(const cr_mx4* m, void* y, cr_row_dtype dtype, long long
 cr_status cr_mx4_gemm(const cr_mx4* x, const cr_mx4* w, const cr_proj_out* outs, int n_outs, void* stream);
 
 /* The same product with the rows of X as they are, [R][ld] of the given type (ld >= w->inner, any alignment of the type): the
- * projections of decode and verify rows, and the head, where the weights' bytes set the time.  Any R in 1..2^20 - 1; made for a few
- * rows, each 25 of them (21 of fp32) read the weights once.  X enters as 4-bit digits: an element is off by at most 2^-30 (fp32:
- * 2^-36) of the power of two above the largest of its block of 32, and what lies under 2^-127 is left out.  The bits of a row do not
- * depend on the other rows of the call nor on their number.  A row that holds an infinity or a NaN gives NaN.  `workspace`: cr_mx4_rows_workspace_bytes(R, w->inner) bytes,
- * 16-byte aligned, of this call alone until it has run.  Bit 6 of the device status word reports a bounded wait that gave up. */
+ * projections of decode and verify rows, and the head, where the weights' bytes set the time.  Any R in 1..2^20 - 1 (R * w->inner
+ * below 2^35, R * w->rows below 2^40); made for a few rows, each 25 of them (21 of fp32) read the weights once.  X enters as 4-bit
+ * digits: an element is off by at most 2^-30 (fp32: 2^-36) of the power of two above the largest of its block of 32, and what lies
+ * under 2^-127 is left out.  The bits of a row do not depend on the other rows of the call nor on their number.  A row that holds
+ * an infinity or a NaN gives NaN.  `workspace`: cr_mx4_rows_workspace_bytes(R, w->inner) bytes, 16-byte aligned, of this call alone
+ * until it has run.  Bit 6 of the device status word reports a bounded wait that gave up. */
 size_t cr_mx4_rows_workspace_bytes(int R, int inner);
 cr_status cr_mx4_rows(const void* x, cr_row_dtype dtype, long long ld, int R, const cr_mx4* w, void* workspace,
                       size_t workspace_bytes, const cr_proj_out* outs, int n_outs, void* stream);

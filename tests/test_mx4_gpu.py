@@ -233,6 +233,22 @@ def test_rows_of_very_large_and_very_small_numbers(dtype):
     check_product(x.double().cpu(), values64(w), [y], 256)
 
 
+def test_rows_of_numbers_near_the_ends_of_the_range():
+    """Rows of numbers down to 2^-126 and up to 2^127 with weights of the other size: what lies under 2^-127 in X is left out, 2^-128 an
+    element."""
+    L = layers()
+    K = 256
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for e, low in ((-126, 220), (-110, 200), (126, 40)):
+        x = (1 + torch.rand(4, K, device="cuda", generator=gen)) * 2.0 ** e * (1 - 2 * torch.randint(0, 2, (4, K), device="cuda", generator=gen))
+        w = random_mx4(64, K, 5, low=low, high=low + 3)
+        y = torch.empty(4, 64, device="cuda")
+        L.mx4_rows(x, w, [y])
+        x64, w64 = x.double().cpu(), values64(w)
+        limit = K * 2.0 ** -24 * (x64.abs() @ w64.abs().t()) + 2.0 ** -127 * w64.abs().sum(1)
+        assert ((y.double().cpu() - x64 @ w64.t()).abs() <= limit).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_rows_with_an_outlier_keep_their_small_elements(dtype):
     """One element 2^13 times the others: the products of the others with it left out of the weights are as exact as ever."""
@@ -248,6 +264,21 @@ def test_rows_with_an_outlier_keep_their_small_elements(dtype):
     x64[:, 100:102] = 0
     want, size = x64 @ values64(w).t(), x64.abs() @ values64(w).abs().t()
     assert ((y.double().cpu() - want).abs() <= 256 * 2.0 ** -24 * size).all()
+
+
+@pytest.mark.parametrize("R", [5, 300])
+def test_scales_of_every_size(R):
+    """Blocks of X and W whose scales go over the whole range of the byte, 0 and 254 among them, and whose products are of one size."""
+    L = layers()
+    K, N = 32 * 256, 96
+    x, w = random_mx4(R, K, 1), random_mx4(N, K, 2)
+    up = (torch.arange(256, device="cuda") * 97 % 255).to(torch.uint8)                  # every value of 0..254 (and one twice)
+    for m, byte in ((x, up), (w, 254 - up)):
+        r, b = torch.arange(m.rows, device="cuda")[:, None], torch.arange(256, device="cuda")[None]
+        m.scales[(r // 128 * 64 + b // 4) * 512 + r % 32 * 16 + r % 128 // 32 * 4 + b % 4] = byte[None].expand(m.rows, 256)
+    y = torch.empty(R, N, device="cuda")
+    L.mx4_gemm(x, w, [y])
+    check_product(values64(x), values64(w), [y], K)
 
 
 @pytest.mark.parametrize("call", ["gemm", "rows"])
