@@ -15,6 +15,15 @@ __device__ __forceinline__ float e8m0(uint32_t b) {
   return __uint_as_float(b == 0 ? 0x00400000u : (b == 255 ? 0x7fc00000u : b << 23));
 }
 
+// The largest magnitude of eight numbers as bits, three at a time; a NaN is above infinity.
+__device__ __forceinline__ uint32_t largest8(const float (&v)[8]) {
+  uint32_t m[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) m[k] = __float_as_uint(v[k]) & 0x7fffffffu;
+  const uint32_t a = __vimax3_u32(m[0], m[1], m[2]), b = __vimax3_u32(m[3], m[4], m[5]);
+  return __vimax3_u32(__vimax3_u32(a, b, m[6]), m[7], 0u);
+}
+
 // Eight numbers times `by` as e2m1 codes: nearest, ties to even, 6 at most.
 __device__ __forceinline__ uint32_t pack_e2m1(const float (&v)[8], float by) {
   uint32_t r;

@@ -3,51 +3,56 @@
 // The exponent field of the largest magnitude is floor(log2) + 127 (0 for a subnormal one, whose s is held to -127 either way), and
 // x 2^-s is exact: both steps have the definition's own bits.
 //
-// HBM-bound: an element's bytes in, 17/32 of a byte out.  A warp takes 256 elements of a row, so that all that depends on the row is
-// computed once for the warp, and four such pieces at a time, asked for before it works on the first.  (With pieces that cross rows
-// each lane found its own row and addresses: 122 instructions for eight elements, and bf16 rows came in at half the rate.)
-// Fp32 rows are stored 16 bytes a lane, a warp's 512 bytes side by side: 32 bytes a lane in two stores were 30 % slower.
+// Fp32 rows are HBM-bound (16,001 x 6,144: 71 us in, 76 us back, 6.1 and 5.0 TB/s); with 16-bit rows the 110 instructions for a lane's eight
+// elements take as long as their bytes (56 and 46 us).  A warp takes 256 elements of a row, so that all that depends on the row is
+// computed once for the warp, and four such pieces at a time, asked for before it works on the first.  With pieces that cross rows each
+// lane found its own row and addresses: 70 us for bf16 rows; with 32 bytes of bf16 a lane 86; fp32 rows stored 32 bytes a lane in two
+// stores instead of a warp's 512 bytes side by side: 110.
 #include "mx4.cuh"
 
 namespace cr {
 
 constexpr int kPieces = 4, kQuantThreads = 256, kQuantPerSm = 16;      // pieces of a warp at a time; CTAs per SM at most
 
-// Piece `i` of `pieces`: row i / segs, elements 256 (i % segs) on.
-struct Piece { int row, seg; };
-__device__ __forceinline__ Piece piece_at(unsigned i, unsigned segs) {
-  const unsigned row = i / segs;
-  return Piece{(int)row, (int)(i - row * segs)};
-}
+// A piece: elements 256 seg .. of a row.  The warp's pieces lie a grid apart and are stepped through, without a division for each.
+struct Piece {
+  int row, seg;
+  __device__ __forceinline__ Piece(unsigned i, unsigned segs) : row((int)(i / segs)), seg((int)(i % segs)) {}
+  __device__ __forceinline__ void step(const Piece& by, int segs) {
+    row += by.row;
+    seg += by.seg;
+    if (seg >= segs) { seg -= segs; ++row; }
+  }
+};
+
+// The warp's first; by a shuffle, which tells the compiler that it is one number for the warp.
+__device__ __forceinline__ unsigned first_piece() { return blockIdx.x * (kQuantThreads / 32) + __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0); }
 
 template <int TYPE>
 __global__ void __launch_bounds__(kQuantThreads) mx4_quant_kernel(const void* __restrict__ x, long long ld, bool wide, uint8_t* __restrict__ codes,
-                                                                  uint8_t* __restrict__ scales, unsigned pieces, int inner) {
+                                                                  uint8_t* __restrict__ scales, int rows, int inner) {
   pdl_release();
   pdl_wait();
-  const unsigned l = threadIdx.x & 31, segs = (inner + 255) / 256, warps = gridDim.x * (kQuantThreads / 32);
-  const int groups = mx4_groups(inner);
-  const unsigned first = blockIdx.x * (kQuantThreads / 32) + __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);      // the warp's, in a uniform register
-  for (unsigned i0 = first; i0 < pieces; i0 += kPieces * warps) {
+  const int l = threadIdx.x & 31, segs = (inner + 255) / 256, groups = mx4_groups(inner);
+  const Piece apart(gridDim.x * (kQuantThreads / 32), segs);
+  for (Piece at(first_piece(), segs); at.row < rows;) {
     float v[kPieces][8];
+    Piece piece[kPieces] = {at, at, at, at};
 #pragma unroll
     for (int k = 0; k < kPieces; ++k) {
-      const unsigned i = i0 + k * warps;
-      const Piece p = piece_at(i, segs);
-      const int col = p.seg * 256 + l * 8;
+      piece[k] = at;
+      const int col = at.seg * 256 + l * 8;
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
-      if (i < pieces && col < inner) load_row8<TYPE>(x, (size_t)p.row * ld + col, wide, v[k]);
+      if (at.row < rows && col < inner) load_row8<TYPE>(x, (size_t)at.row * ld + col, wide, v[k]);
+      at.step(apart, segs);
     }
 #pragma unroll
     for (int k = 0; k < kPieces; ++k) {
-      const unsigned i = i0 + k * warps;
-      if (i >= pieces) break;
-      const Piece p = piece_at(i, segs);
+      const Piece p = piece[k];
+      if (p.row >= rows) break;
       const int col = p.seg * 256 + l * 8;
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[k][j]) & 0x7fffffffu);
+      uint32_t top = largest8(v[k]);
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int field = (int)(top >> 23);                            // 255: an infinity or a NaN is among them
@@ -62,36 +67,35 @@ __global__ void __launch_bounds__(kQuantThreads) mx4_quant_kernel(const void* __
 }
 
 template <int TYPE>
-__global__ void __launch_bounds__(kQuantThreads) mx4_dequant_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, unsigned pieces, int inner,
+__global__ void __launch_bounds__(kQuantThreads) mx4_dequant_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, int inner,
                                                                     void* __restrict__ y, long long ld, bool wide) {
   constexpr int PER = TYPE == CR_ROW_F32 ? 4 : 8, PARTS = 8 / PER;   // elements of a lane that lie together: 16 bytes of the row
   pdl_release();
   pdl_wait();
-  const unsigned l = threadIdx.x & 31, segs = (inner + 255) / 256, warps = gridDim.x * (kQuantThreads / 32);
-  const int groups = mx4_groups(inner);
-  const unsigned first = blockIdx.x * (kQuantThreads / 32) + __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
-  for (unsigned i0 = first; i0 < pieces; i0 += kPieces * warps) {
+  const int l = threadIdx.x & 31, segs = (inner + 255) / 256, groups = mx4_groups(inner);
+  const Piece apart(gridDim.x * (kQuantThreads / 32), segs);
+  for (Piece at(first_piece(), segs); at.row < rows;) {
     uint32_t w[kPieces][PARTS], byte[kPieces][PARTS];
+    Piece piece[kPieces] = {at, at, at, at};
 #pragma unroll
     for (int k = 0; k < kPieces; ++k) {
-      const unsigned i = i0 + k * warps;
-      const Piece p = piece_at(i, segs);
+      piece[k] = at;
 #pragma unroll
       for (int h = 0; h < PARTS; ++h) {
-        const int at = h * 128 + l * PER, col = p.seg * 256 + at, block = at / 32;
+        const int in = h * 128 + l * PER, col = at.seg * 256 + in, block = in / 32;
         w[k][h] = byte[k][h] = 0;
-        if (i < pieces && col < inner) {
-          const uint8_t* c = codes + (size_t)p.row * (inner / 2) + col / 2;
+        if (at.row < rows && col < inner) {
+          const uint8_t* c = codes + (size_t)at.row * (inner / 2) + col / 2;
           w[k][h] = PER == 8 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
-          byte[k][h] = scales[mx4_scale_at(p.row, p.seg * 8, groups) + (block >> 2) * 512 + (block & 3)];
+          byte[k][h] = scales[mx4_scale_at(at.row, at.seg * 8, groups) + (block >> 2) * 512 + (block & 3)];
         }
       }
+      at.step(apart, segs);
     }
 #pragma unroll
     for (int k = 0; k < kPieces; ++k) {
-      const unsigned i = i0 + k * warps;
-      if (i >= pieces) break;
-      const Piece p = piece_at(i, segs);
+      const Piece p = piece[k];
+      if (p.row >= rows) break;
 #pragma unroll
       for (int h = 0; h < PARTS; ++h) {
         const int col = p.seg * 256 + h * 128 + l * PER;
@@ -134,12 +138,11 @@ __global__ void __launch_bounds__(kQuantThreads) mx4_dequant_kernel(const uint8_
   }
 }
 
-// Pieces of a matrix, and the CTAs that take them.
-static cr_status quant_grid(const cr_mx4* m, const char* who, unsigned* pieces, dim3* grid) {
+// The CTAs that take a matrix.
+static cr_status quant_grid(const cr_mx4* m, const char* who, dim3* grid) {
   const long long all = (long long)m->rows * ((m->inner + 255) / 256);
   CR_REQUIRE(all < (1ll << 31), "%s: %d x %d elements are too many for a call", who, m->rows, m->inner);
   const long long ctas = (all + kQuantThreads / 32 - 1) / (kQuantThreads / 32), most = (long long)sm_count() * kQuantPerSm;
-  *pieces = (unsigned)all;
   *grid = dim3((unsigned)(ctas < most ? ctas : most));
   return CR_OK;
 }
@@ -155,13 +158,12 @@ extern "C" cr_status cr_mx4_quant(const void* x, cr_row_dtype dtype, long long l
   using namespace cr;
   if (cr_status s = check_mx4(to, "cr_mx4_quant", "destination")) return s;
   if (cr_status s = check_rows(x, dtype, ld, to->inner, "cr_mx4_quant")) return s;
-  unsigned pieces;
   dim3 grid;
-  if (cr_status s = quant_grid(to, "cr_mx4_quant", &pieces, &grid)) return s;
+  if (cr_status s = quant_grid(to, "cr_mx4_quant", &grid)) return s;
   cudaStream_t stream = (cudaStream_t)stream_;
   use_stream(stream);
   return by_dtype(dtype, [&](auto type) -> cr_status {
-    CR_CUDA(launch_pdl(mx4_quant_kernel<decltype(type)::value>, grid, dim3(kQuantThreads), 0, stream, x, ld, wide_rows(x, dtype, ld), to->codes, to->scales, pieces,
+    CR_CUDA(launch_pdl(mx4_quant_kernel<decltype(type)::value>, grid, dim3(kQuantThreads), 0, stream, x, ld, wide_rows(x, dtype, ld), to->codes, to->scales, to->rows,
                        to->inner));
     CR_LAUNCH_CHECK("mx4_quant_kernel");
     return CR_OK;
@@ -172,13 +174,12 @@ extern "C" cr_status cr_mx4_dequant(const cr_mx4* m, void* y, cr_row_dtype dtype
   using namespace cr;
   if (cr_status s = check_mx4(m, "cr_mx4_dequant", "matrix")) return s;
   if (cr_status s = check_rows(y, dtype, ld, m->inner, "cr_mx4_dequant")) return s;
-  unsigned pieces;
   dim3 grid;
-  if (cr_status s = quant_grid(m, "cr_mx4_dequant", &pieces, &grid)) return s;
+  if (cr_status s = quant_grid(m, "cr_mx4_dequant", &grid)) return s;
   cudaStream_t stream = (cudaStream_t)stream_;
   use_stream(stream);
   return by_dtype(dtype, [&](auto type) -> cr_status {
-    CR_CUDA(launch_pdl(mx4_dequant_kernel<decltype(type)::value>, grid, dim3(kQuantThreads), 0, stream, m->codes, m->scales, pieces, m->inner, y, ld,
+    CR_CUDA(launch_pdl(mx4_dequant_kernel<decltype(type)::value>, grid, dim3(kQuantThreads), 0, stream, m->codes, m->scales, m->rows, m->inner, y, ld,
                        wide_rows(y, dtype, ld)));
     CR_LAUNCH_CHECK("mx4_dequant_kernel");
     return CR_OK;
