@@ -33,14 +33,17 @@ CR_DEFINE_STATUS_WORD(mx4_rows)
 
 constexpr int kDigitsMost = 12, kPassRows = 256;                 // digit rows of a pass over W
 __host__ __device__ constexpr int digits_of(int dtype) { return dtype == CR_ROW_F32 ? 12 : 10; }
-constexpr int kRowsMost = kPassRows / digits_of(CR_ROW_BF16);    // rows of X of a pass
+// Digit rows come in halves of 128: so many rows of X fill one, twice as many make a pass.
+__host__ __device__ constexpr int half_rows(int digits) { return 128 / digits; }
+constexpr int kHalfMost = half_rows(10);
+__host__ __device__ constexpr int digit_row(int r, int digits) { return r / half_rows(digits) * 128 + r % half_rows(digits) * digits; }
 constexpr int kStream = -1;                                      // digits from the workspace, instead of from rows of a type
 // producer, issuer, four epilogue warps; eight where they make digits before
 __host__ __device__ constexpr int rows_threads(int from) { return from == kStream ? 192 : 320; }
 constexpr int kOwnElements = 2048;                               // elements of X that a CTA turns into digits itself
 constexpr int kNMaxStages = 8;
 constexpr size_t kNRing = 212992;
-constexpr size_t kNSmem = kNRing + (2 * kNMaxStages + 5) * 8 + 16;
+constexpr size_t kNSmem = kNRing + (2 * kNMaxStages + 6) * 8 + 16;
 
 // ---- digits ----------------------------------------------------------------------------------------------------------
 // The digits of eight elements of a block, whose other elements are with three neighbouring threads (`quad`: the four lanes): for each
@@ -86,7 +89,7 @@ __global__ void __launch_bounds__(128) mx4_digits_kernel(const void* __restrict_
   const int row = (int)(u / per_row), i = (int)(u - (long long)row * per_row);
   float v[8];
   load_row8<TYPE>(x, (size_t)row * ld + (size_t)i * 8, wide, v);
-  const int at = row / pass_rows * kPassRows + row % pass_rows * digits_of(TYPE);
+  const int at = row / pass_rows * kPassRows + digit_row(row % pass_rows, digits_of(TYPE));
   uint32_t* to = reinterpret_cast<uint32_t*>(codes) + (size_t)at * per_row + i;
   make_digits<digits_of(TYPE)>(v, 0xfu << (threadIdx.x & 28), [&](int j, uint32_t word, uint8_t scale) {
     to[(size_t)j * per_row] = word;
@@ -107,6 +110,11 @@ struct RowsShape {
 // Columns of tensor memory: an accumulator's (read 16 at a time from a row's first digit on) and the scales' of a stage.
 __host__ __device__ inline int acc_columns(int cols) { return (cols + 31) / 32 * 32; }
 __host__ __device__ inline int scale_columns(int cols) { return cols > 128 ? 24 : 16; }
+
+// The same for CTA pairs: from one accumulator to the other, and the first scale column.
+__host__ __device__ inline bool pair_shares(int cols) { return cols > 192; }
+__host__ __device__ inline int pair_acc_step(int cols) { return pair_shares(cols) ? 128 : acc_columns(cols); }
+__host__ __device__ inline int pair_scale_column(int cols) { return pair_shares(cols) ? 384 : 2 * acc_columns(cols); }
 
 template <int FROM>
 __global__ void __launch_bounds__(rows_threads(FROM), 1)
@@ -251,12 +259,14 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
       umma::fence_after_sync();
       int o = 0;
       while (o < P.n_outs - 1 && n0 >= P.col0[o] + P.cols[o]) ++o;     // 32 columns never straddle outputs
-      float y[kRowsMost];
+      const int half = 128 / S.digits;
+      float y[2 * kHalfMost];
 #pragma unroll
-      for (int r = 0; r < kRowsMost; ++r) {
+      for (int r = 0; r < 2 * kHalfMost; ++r) {
         if (r >= live) break;
         float v[16];
-        umma::tmem_ld16(umma::tmem_addr(tm, q, a * acc_cols + r * S.digits), v);     // warp-collective
+        const int col = r < half ? r * S.digits : 128 + (r - half) * S.digits;
+        umma::tmem_ld16(umma::tmem_addr(tm, q, a * acc_cols + col), v);     // warp-collective
         y[r] = 0.f;
 #pragma unroll
         for (int j = kDigitsMost - 1; j >= 0; --j)
@@ -266,7 +276,7 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
       __syncwarp();
       if (l == 0) umma::mbar_arrive_relaxed(&accEmpty[a]);                  // the next tile's products may come
 #pragma unroll
-      for (int r = 0; r < kRowsMost; ++r) {
+      for (int r = 0; r < 2 * kHalfMost; ++r) {
         if (r >= live) break;
         if (S.splits > 1) {
           reinterpret_cast<float*>(sm)[r * 128 + 32 * q + l] = y[r];                  // every stage has been read
@@ -301,6 +311,167 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
   cluster.sync();                                                       // the parts stay until everybody has read them
 }
 
+// ---- many digit rows: CTA pairs over two tiles of W ---------------------------------------------------------------------
+// With more than 128 digit rows a CTA's shared memory sets the pace (see mx4_gemm_pair_kernel): a pair multiplies 256 rows of W, each CTA
+// its 128, with all digit rows, each CTA half of them.  Whole accumulators in turn up to 192 digit rows; above, two that share 128
+// columns, which are free once the warps of that half have read them.  Stage: codes of W, half of X's codes, scales of W, all of X's
+// scales.  D: digits of an element.
+constexpr int kPairThreads = 64 + 256;                           // producer, issuer, four epilogue warps to each half of the digit rows
+template <int D>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+mx4_rows_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ RowsShape S, const __grid_constant__ CUtensorMap wmap,
+                     const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wsmap, const __grid_constant__ CUtensorMap xsmap) {
+  extern __shared__ __align__(1024) unsigned char sm[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kNRing);
+  uint64_t *full = bars, *empty = bars + kNMaxStages, *accFull = bars + 2 * kNMaxStages, *handed = bars + 2 * kNMaxStages + 2;     // handed: [accumulator][half]
+  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 2 * kNMaxStages + 6);
+  volatile int& dead = *reinterpret_cast<volatile int*>(&tmem_slot + 1);
+  cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t rank = cluster.block_rank();                          // 0 leads
+  const int t = threadIdx.x, w = t >> 5, l = t & 31;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1, units = S.tiles * S.passes, kb_n = (P.K + kXK - 1) / kXK, ST = S.stages;
+  const bool shared = pair_shares(S.cols);
+  const int xcodes = S.cols / 2 * (kXK / 2);
+  if (t == 0) {
+    for (int i = 0; i < ST; ++i) { umma::mbar_init(&full[i], 1); umma::mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2; ++i) umma::mbar_init(&accFull[i], 1);
+    for (int i = 0; i < 4; ++i) umma::mbar_init(&handed[i], 8);           // four epilogue warps in each CTA
+    umma::mbar_fence_init();
+    dead = (umma::smem_u32(sm) & 1023u) != 0;                           // the swizzled tiles need 1 KB boundaries
+    if (dead) g_mx4_rows_status = 1;
+    prefetch_map(&wmap); prefetch_map(&xmap); prefetch_map(&wsmap); prefetch_map(&xsmap);
+  }
+  if (w == 1) umma::pair_tmem_alloc(&tmem_slot, 512);
+  umma::fence_before_sync();
+  cluster.sync();                                                       // both CTAs' barriers are ready
+  umma::fence_after_sync();
+  pdl_release();
+  const uint32_t tm = tmem_slot;
+  bool gave_up = dead;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (gave_up) return;
+    if (!umma::mbar_wait_timed(bar, parity, &dead)) { gave_up = true; dead = 1; g_mx4_rows_status = 1; }
+  };
+  int issued = 0;
+  if (w == 0) {
+    if (l == 0) {
+      struct Cursor {
+        int unit, left, kb, n0, pass, s, phase;
+        __device__ __forceinline__ void seek(int passes) { n0 = unit / passes; pass = unit - n0 * passes; n0 *= 256; }
+      };
+      const int all = first < units ? (units - first + step - 1) / step * kb_n : 0;
+      auto advance = [&](Cursor& c) {
+        --c.left;
+        if (++c.kb == kb_n) { c.kb = 0; c.unit += step; c.seek(S.passes); }
+        if (++c.s == ST) { c.s = 0; c.phase ^= 1; }
+      };
+      auto load_w = [&](const Cursor& c) {
+        unsigned char* st = sm + c.s * S.stage;
+        if (rank == 0) umma::mbar_expect_tx(&full[c.s], 2 * S.stage);
+        const uint32_t bar = umma::cluster_addr(&full[c.s], 0);
+        pair_load_box_2d(st, &wmap, c.kb * (kXK / 2), c.n0 + 128 * (int)rank, bar);
+        pair_load_box_2d(st + kXTile + xcodes, &wsmap, c.kb * 256, c.n0 / 128 + (int)rank, bar);
+      };
+      auto load_x = [&](const Cursor& c) {
+        unsigned char* st = sm + c.s * S.stage + kXTile;
+        const uint32_t bar = umma::cluster_addr(&full[c.s], 0);
+        pair_load_box_2d(st, &xmap, c.kb * (kXK / 2), c.pass * kPassRows + S.cols / 2 * (int)rank, bar);
+        pair_load_box_2d(st + xcodes + kXScale, &xsmap, c.kb * 256, c.pass * (kPassRows / 128), bar);
+      };
+      Cursor cw{first, all, 0, 0, 0, 0, 0};
+      cw.seek(S.passes);
+      Cursor cx = cw;
+      for (int i = 0; i < ST && cw.left > 0; ++i) { load_w(cw); advance(cw); }
+      pdl_wait();
+      for (int i = 0; i < ST && cx.left > 0; ++i) { load_x(cx); advance(cx); }
+      while (cw.left > 0) {
+        wait(&empty[cw.s], cw.phase ^ 1);
+        if (gave_up) break;
+        load_w(cw);
+        load_x(cw);
+        advance(cw);
+      }
+      issued = all - cw.left;
+    }
+  } else if (w == 1) {
+    if (rank == 0) {
+      const bool one = elect_one();
+      const Desc wc(tma::desc_sw128(sm, 16, 1024)), xc(tma::desc_sw128(sm + kXTile, 16, 1024));
+      const Desc ws(umma::smem_desc(sm + kXTile + xcodes, 0, 128)), xs(umma::smem_desc(sm + kXTile + xcodes + kXScale, 0, 128));
+      const uint32_t idesc = idesc_mx4(256, S.cols), scales = tm + pair_scale_column(S.cols);
+      int s = 0, phase = 0, local = 0;
+      for (int u = first; u < units && !gave_up; u += step, ++local) {
+        const int odd = local & 1;
+        const uint32_t acc = tm + odd * pair_acc_step(S.cols);
+        if (local >= 2) {                                                  // this accumulator has been read
+          wait(&handed[2 * odd], ((local - 2) >> 1) & 1);
+          wait(&handed[2 * odd + 1], ((local - 2) >> 1) & 1);
+        }
+        // and the shared columns of the other one: the second half of the even accumulator, the first half of the odd one
+        if (shared && local >= 1) wait(&handed[2 * (odd ^ 1) + odd], ((local - 1) >> 1) & 1);
+        for (int kb = 0; kb < kb_n; ++kb) {
+          wait(&full[s], phase);
+          if (gave_up) break;
+          umma::fence_after_sync();
+          const uint32_t off = s * (S.stage / 16), cols = scales + s * 24;
+          const int steps = P.K / 64 - kb * 4;
+          if (one) {
+            issue_scales<2, 2>(cols, ws, off, xs, off, steps);
+            issue_products<2, 2>(acc, wc, off, xc, off, cols, 0, idesc, steps, kb == 0);
+            umma::pair_commit(&empty[s]);                                         // the stage is free in both CTAs once these products have read it
+            if (kb == kb_n - 1) umma::pair_commit(&accFull[odd]);
+          }
+          if (++s == ST) { s = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else {
+    constexpr int HALF = half_rows(D), GROUP = HALF / 2;                 // rows of X of a half; of one read of 64 columns
+    static_assert(GROUP * D <= 64 && 2 * GROUP == HALF, "");
+    const int q = w & 3, h = (w - 2) >> 2;
+    int local = 0;
+    for (int u = first; u < units; u += step, ++local) {
+      const int odd = local & 1, n0 = u / S.passes * 256 + 128 * (int)rank + 32 * q;
+      const int r0 = u % S.passes * S.pass_rows + h * HALF, live = min(HALF, min(S.pass_rows - h * HALF, P.R - r0));   // rows of this half
+      if (l == 0) wait(&accFull[odd], (local >> 1) & 1);
+      __syncwarp();
+      if (dead) break;
+      umma::fence_after_sync();
+      float y[HALF];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        if (g * GROUP >= live) break;
+        float v[64];
+        umma::tmem_ld64(umma::tmem_addr(tm, q, odd * pair_acc_step(S.cols) + 128 * h + g * GROUP * D), v);     // warp-collective
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i) {
+          y[g * GROUP + i] = 0.f;
+#pragma unroll
+          for (int j = D - 1; j >= 0; --j) y[g * GROUP + i] += v[i * D + j];
+        }
+      }
+      umma::fence_before_sync();
+      __syncwarp();
+      if (l == 0) umma::pair_arrive_relaxed(umma::cluster_addr(&handed[2 * odd + h], 0));
+      if (n0 >= P.N) continue;
+      int o = 0;
+      while (o < P.n_outs - 1 && n0 >= P.col0[o] + P.cols[o]) ++o;       // 32 columns never straddle outputs
+#pragma unroll
+      for (int i = 0; i < HALF; ++i) {
+        if (i >= live) break;
+        const size_t at = (size_t)(r0 + i) * P.ld[o] + (n0 + l - P.col0[o]);
+        if (P.f32[o]) reinterpret_cast<float*>(P.ptr[o])[at] = y[i];
+        else reinterpret_cast<__nv_bfloat16*>(P.ptr[o])[at] = __float2bfloat16_rn(y[i]);
+      }
+    }
+  }
+  if (dead && rank == 0 && w == 0 && l == 0) drain_copies(full, issued, ST);     // both CTAs' copies complete on the leader's barriers
+  umma::fence_before_sync();
+  __syncwarp();
+  cluster.sync();                                                          // neither CTA leaves while the other may still use its memory
+  if (w == 1) umma::pair_tmem_dealloc(tm, 512);
+}
+
 // CTAs that share K: as many as give every SM a tile, while all clusters run at once.  R has no part in it.
 static cr_status rows_splits(int N, int K, int* splits) {
   static PerDeviceOnce configured;
@@ -312,6 +483,8 @@ static cr_status rows_splits(int N, int K, int* splits) {
         CR_CUDA(cudaFuncSetAttribute(mx4_rows_kernel<CR_ROW_F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kNSmem));
         CR_CUDA(cudaFuncSetAttribute(mx4_rows_kernel<CR_ROW_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kNSmem));
         CR_CUDA(cudaFuncSetAttribute(mx4_rows_kernel<CR_ROW_F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kNSmem));
+        CR_CUDA(cudaFuncSetAttribute(mx4_rows_pair_kernel<10>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kNSmem));
+        CR_CUDA(cudaFuncSetAttribute(mx4_rows_pair_kernel<12>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kNSmem));
         for (int s = 1; s <= 8; ++s) {
           cudaLaunchConfig_t cfg = {};
           cfg.gridDim = dim3(s); cfg.blockDim = dim3(rows_threads(kStream)); cfg.dynamicSmemBytes = kNSmem;
@@ -353,9 +526,9 @@ static cr_status rows_launch(const ProjParams& P, const RowsShape& S, const CUte
 
 }  // namespace cr
 
-// Passes over W of R rows: as few as hold them, with as many rows in each.
+// Passes over W of R rows: as few as hold them, with about as many rows in each.
 static int rows_passes(int R, int digits) {
-  const int most = cr::kPassRows / digits;
+  const int most = 2 * cr::half_rows(digits);
   return (R + most - 1) / most;
 }
 extern "C" size_t cr_mx4_rows_workspace_bytes(int R, int inner) {
@@ -381,16 +554,19 @@ extern "C" cr_status cr_mx4_rows(const void* x, cr_row_dtype dtype, long long ld
   S.digits = digits_of(dtype);
   S.passes = rows_passes(R, S.digits);
   S.pass_rows = (R + S.passes - 1) / S.passes;
-  S.cols = (S.digits * S.pass_rows + 7) / 8 * 8;
+  // A multiple of 16 above 128: a pair halves it.
+  S.cols = S.pass_rows <= half_rows(S.digits) ? (S.digits * S.pass_rows + 7) / 8 * 8 : (digit_row(S.pass_rows - 1, S.digits) + S.digits + 15) / 16 * 16;
+  const bool pairs = S.splits == 1 && S.cols > 128;
   cr_mx4 d{static_cast<uint8_t*>(workspace), nullptr, S.passes * kPassRows, w->inner};
   d.scales = d.codes + cr_mx4_code_bytes(d.rows, d.inner);
   const int kb_most = ((w->inner + kXK - 1) / kXK + S.splits - 1) / S.splits;
   const bool own = S.passes == 1 && S.cols <= 128 && (long long)R * kb_most * kXK <= kOwnElements;
-  S.stage = kXTile + kXScale + (own ? 0 : S.cols * (kXK / 2) + (S.cols > 128 ? 2 : 1) * kXScale);
+  S.stage = kXTile + kXScale + (own ? 0 : S.cols / (pairs ? 2 : 1) * (kXK / 2) + (S.cols > 128 ? 2 : 1) * kXScale);
   const size_t room = kNRing - (own ? (size_t)kb_most * (S.cols * (kXK / 2) + kXScale) : 0);
   // Two accumulators while they leave columns for the scales of four stages: the epilogue of a tile beside the products of the next.
   S.accs = 2 * acc_columns(S.cols) + 4 * scale_columns(S.cols) <= 512 ? 2 : 1;
-  const int columned = (512 - S.accs * acc_columns(S.cols)) / scale_columns(S.cols), most = columned < kNMaxStages ? columned : kNMaxStages;
+  const int columned = (512 - (pairs ? pair_scale_column(S.cols) : S.accs * acc_columns(S.cols))) / scale_columns(S.cols);
+  const int most = columned < kNMaxStages ? columned : kNMaxStages;
   S.stages = (int)(room / S.stage) < most ? (int)(room / S.stage) : most;
   S.x = x;
   S.ld = ld;
@@ -404,7 +580,7 @@ extern "C" cr_status cr_mx4_rows(const void* x, cr_row_dtype dtype, long long ld
     maps[3] = maps[2];
     return by_dtype(dtype, [&](auto type) { return rows_launch<decltype(type)::value>(P, S, maps, stream); });
   }
-  if (cr_status s = map_mx4(&maps[1], &maps[3], &d, S.cols, S.cols > 128 ? 2 : 1)) return s;
+  if (cr_status s = map_mx4(&maps[1], &maps[3], &d, S.cols / (pairs ? 2 : 1), S.cols > 128 ? 2 : 1)) return s;
   if (cr_status s = by_dtype(dtype, [&](auto type) -> cr_status {
         const long long threads = (long long)R * (w->inner / 8);
         CR_CUDA(launch_pdl(mx4_digits_kernel<decltype(type)::value>, dim3((unsigned)((threads + 127) / 128)), dim3(128), 0, stream, x, ld, (bool)S.wide, d.codes, d.scales,
@@ -412,5 +588,12 @@ extern "C" cr_status cr_mx4_rows(const void* x, cr_row_dtype dtype, long long ld
         CR_LAUNCH_CHECK("mx4_digits_kernel");
         return CR_OK;
       })) return s;
-  return rows_launch<kStream>(P, S, maps, stream);
+  if (!pairs) return rows_launch<kStream>(P, S, maps, stream);
+  S.tiles = (P.N + 255) / 256;
+  const long long units = (long long)S.tiles * S.passes;
+  const int most_pairs = sm_count() / 2;
+  CR_CUDA(launch_pdl(S.digits == 10 ? mx4_rows_pair_kernel<10> : mx4_rows_pair_kernel<12>, dim3(2 * (unsigned)(units < most_pairs ? units : most_pairs)), dim3(kPairThreads), kNSmem, stream, P, S, maps[0], maps[1],
+                     maps[2], maps[3]));
+  CR_LAUNCH_CHECK("mx4_rows_pair_kernel");
+  return CR_OK;
 }

@@ -196,6 +196,14 @@ def test_product_of_two_4_bit_matrices(R, K, widths, f32):
     (33, 1088, [544], [False]),
     (72, 2048, [8224], [True]),
     (100, 256, [128], [True]),
+    (11, 320, [9632], [True]),                                   # more tiles than a wave of clusters, by the number of digit rows:
+    (13, 576, [9568, 32], [False, True]),
+    (17, 192, [9632], [True]),
+    (20, 1088, [9600, 64], [True, False]),
+    (21, 512, [9632], [True]),
+    (24, 320, [9632], [True]),
+    (25, 448, [9760], [True]),
+    (50, 192, [19232], [True]),                                  # several tiles a pair, several passes
 ])
 def test_product_of_rows_as_they_are(R, K, widths, f32, dtype):
     L = layers()
@@ -215,7 +223,7 @@ def test_a_row_has_the_same_bits_in_every_call(K, N, dtype):
     x = torch.randn(45, K, device="cuda").to(dtype)
     whole = torch.empty(45, N, device="cuda")
     L.mx4_rows(x, w, [whole])
-    for r0, n in ((0, 1), (3, 2), (5, 4), (7, 8), (11, 13), (20, 20), (44, 1)):
+    for r0, n in ((0, 1), (3, 2), (5, 4), (7, 8), (11, 13), (20, 20), (20, 24), (1, 16), (44, 1)):
         part = torch.empty(n, N, device="cuda")
         L.mx4_rows(x[r0:r0 + n], w, [part])
         assert torch.equal(part, whole[r0:r0 + n])
