@@ -11,17 +11,21 @@
 // nothing from them.  The sums of an output's digits, each in fp32, are added from the smallest up.  The order of all sums depends on N
 // and K alone: a row has the same bits in every call.
 //
-// mx4_rows_kernel: 128 rows of W are the M side, up to 256 digit rows the N side; persistent over W, or one tile per cluster of CTAs that
-// share K where there are few tiles.  With few elements of X for a CTA it makes their digits itself, into the tiles that the
+// mx4_rows_kernel: 128 rows of W are the M side, up to 256 digit rows the N side; persistent over W (up to 128 digit rows), or one tile
+// per cluster of CTAs that share K where there are few tiles.  With few elements of X for a CTA it makes their digits itself, into the tiles that the
 // tensor cores read, while the first stages of W arrive: one launch.  Otherwise mx4_digits_kernel writes them into the workspace, a
 // block of 256 rows for each pass over W, from where they come with every stage, and the first stages of W are asked for while it runs.
 // The line between the two is at 2,048 elements: 1 x 2,048 x 12,352 takes 6.1 us this way and 7.9 that way, 1 x 4,096 x 2,048 (eight CTAs
 // to a row) 6.5 and 7.2; 2 x 2,048 x 131,072 29.3 and 29.0, 4 x 2,048 x 12,352 11.5 and 8.4, since every CTA makes all digits.
 //
+// mx4_rows_pair_kernel, for more than 128 digit rows where nothing shares K: CTA pairs, 256 rows of W to a tile, each CTA with half of the
+// digits' codes, which come from L2 once for 256 rows of W and not for 128.  At 131,072 x 2,048, against one CTA: 16 rows 30.9 and 32.8 us,
+// 20 rows 33.7 and 47.9, 24 rows 35.3 and 52.9, 72 rows (three passes) 79.6 and 131.7.
+//
 // What bounds it: W at 131,072 x 2,048 is 142.6 MB, 21.8 us at the copy bandwidth and 22.6 us for the same copies without products.  One row
-// takes 26.3 us, 9 rows 30.8, 13 rows 32.2 (4.6 TB/s): the launches, the first stage's and the last tile's latency, 4 to 7 us.  The
+// takes 26.3 us, 9 rows 30.5, 13 rows 30.1 (4.9 TB/s): the launches, the first stage's and the last tile's latency, 4 to 7 us.  The
 // copying thread's divisions had cost 4 us; one accumulator for 11 to 19 rows 13 us, since the epilogue stands between two tiles then.
-// 20 to 25 rows have one (48 to 54 us).  Calls over few weights are latencies: 1 x 64 x 32 3.6 us.
+// Calls over few weights are latencies: 1 x 64 x 32 3.6 us.
 #include <cooperative_groups.h>
 #include "mx4_mma.cuh"
 
