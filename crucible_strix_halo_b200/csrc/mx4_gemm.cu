@@ -3,7 +3,7 @@
 //
 // A step of 64 moves the bytes of a bf16 step of 16 in the same cycles, so the kernels are shaped as those of cr_proj_gemm.
 //
-// mx4_gemm_pair_kernel (many rows): CTA pairs on 256 x 256 tiles.  Two accumulators of 256 columns would fill tensor memory and
+// mx4_gemm_pair_kernel<PARTS> (many rows): CTA pairs on 256 x 256 tiles.  Two accumulators of 256 columns would fill tensor memory and
 // leave the scales no room: they share 128 columns, which the epilogue reads first and hands over before it stores.  The issuing warp
 // decides the pace: with one lane in a branch of its own its descriptors went through vector registers and 32,768 x 2,048 x 12,352
 // took 566 us (no stores: 496); with all lanes in the loop and one elected for the instructions 442 (296).  Rows turned through shared
@@ -11,6 +11,8 @@
 // rate.  What bounds it now is the power cap: block after block of calls runs at 1.3 GHz and takes 416 us (the same products without
 // stores 332 us at 1.57 GHz); short K the stores (16,384 x 64 x 12,800: 5.1 TB/s).  Taken back: two whole accumulators on 256 x 192
 // tiles (384 us: more bytes a product), stores by the copy engine (387), waits that spin (K = 6,144: 103 -> 109 us).
+// The few tiles of a last wave are cut into PARTS = 2 or 4, of 128 or 64 columns: 2,048 x 2,048 x 9,856 (312 tiles for 74 pairs) 28.8 -> 27.7 us,
+// 2,500 x 512 x 6,144 (240) 19.6 -> 17.7, 8,192 x 2,048 x 2,048 (256) 21.4 -> 20.6.
 //
 // mx4_gemm_split_kernel<TN> (few rows): 128 x TN tiles, K split over a cluster of up to eight CTAs, bound by latencies: 333 x 4,096 x 2,048
 // takes 7.9 us, 1 x 64 x 32 2.1 us.
@@ -82,9 +84,14 @@ static_assert(kQStages * 24 <= kQShared, "every stage has scale columns of its o
 constexpr int kQTurn = kQStages * kQStageBytes;                            // room of the epilogue warps behind the stages
 constexpr size_t kQSmem = (size_t)kQTurn + kQWarps * kTurnBytes + (2 * kQStages + 4) * 8 + 16;
 
+// Tiles that are left after the last full wave are cut into this many, of as many columns each, while every part finds a pair.
+constexpr int pair_parts(long long left, int pairs) { return left == 0 ? 1 : 4 * left <= pairs ? 4 : 2 * left <= pairs ? 2 : 1; }
+
+// whole: tiles that are not cut; cmap: codes of W in boxes for the parts of the others.
+template <int PARTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kQThreads, 1)
 mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
-                     const __grid_constant__ CUtensorMap xsmap, const __grid_constant__ CUtensorMap wsmap) {
+                     const __grid_constant__ CUtensorMap cmap, const __grid_constant__ CUtensorMap xsmap, const __grid_constant__ CUtensorMap wsmap, int whole) {
   extern __shared__ __align__(1024) unsigned char sm[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kQTurn + kQWarps * kTurnBytes);
   uint64_t *full = bars, *empty = bars + kQStages, *accFull = bars + 2 * kQStages, *handed = bars + 2 * kQStages + 2;
@@ -94,12 +101,20 @@ mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant
   const uint32_t rank = cluster.block_rank();                          // 0 leads
   const int t = threadIdx.x, w = t >> 5, l = t & 31;
   const int mt = (P.R + 255) / 256, nt = (P.N + 255) / 256, kb_n = (P.K + kXK - 1) / kXK, tiles = mt * nt;
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  auto tile_at = [&](int i, int& m0, int& n0) {
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, units = PARTS == 1 ? tiles : whole + (tiles - whole) * PARTS;
+  // Unit i: a tile, or columns from..from + width - 1 of one.
+  auto unit_at = [&](int i, int& m0, int& n0, int& from, int& width) {
+    from = 0;
+    width = 256;
+    if (PARTS > 1 && i >= whole) {
+      width = 256 / PARTS;
+      from = (i - whole) % PARTS * width;
+      i = whole + (i - whole) / PARTS;
+    }
     const int per_band = mt * kQBand, band = i / per_band, in = i - band * per_band;
-    const int width = min(kQBand, nt - band * kQBand);
-    m0 = (in / width) * 256;
-    n0 = (band * kQBand + in % width) * 256;
+    const int tiles_wide = min(kQBand, nt - band * kQBand);
+    m0 = (in / tiles_wide) * 256;
+    n0 = (band * kQBand + in % tiles_wide) * 256;
   };
   if (t == 0) {
     for (int i = 0; i < kQStages; ++i) { umma::mbar_init(&full[i], 1); umma::mbar_init(&empty[i], 1); }
@@ -128,17 +143,20 @@ mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant
     // ---------------------------------------------------------------- producer (each CTA its own rows of X and of W, all of W's scales)
     if (l == 0) {
       int s = 0, phase = 1;
-      for (int i = pair; i < tiles && !gave_up; i += pairs) {
-        int m0, n0;
-        tile_at(i, m0, n0);
+      for (int i = pair; i < units && !gave_up; i += pairs) {
+        int m0, n0, from, width;
+        unit_at(i, m0, n0, from, width);
+        const uint32_t bytes = 2 * kQStageBytes - (256 - width) * (kXK / 2);
+        const CUtensorMap* codes = PARTS == 1 || width == 256 ? &wmap : &cmap;
+        const int wrow = n0 + from + width / 2 * (int)rank;
         for (int kb = 0; kb < kb_n; ++kb, ++issued) {
           if (issued >= kQStages) wait(&empty[s], phase);
           if (gave_up) break;
           unsigned char* st = sm + s * kQStageBytes;
-          if (rank == 0) umma::mbar_expect_tx(&full[s], 2 * kQStageBytes);
+          if (rank == 0) umma::mbar_expect_tx(&full[s], bytes);
           const uint32_t bar = umma::cluster_addr(&full[s], 0);
           pair_load_box_2d(st, &xmap, kb * (kXK / 2), m0 + 128 * (int)rank, bar);
-          pair_load_box_2d(st + kXTile, &wmap, kb * (kXK / 2), n0 + 128 * (int)rank, bar);
+          pair_load_box_2d(st + kXTile, codes, kb * (kXK / 2), wrow, bar);
           pair_load_box_2d(st + 2 * kXTile, &xsmap, kb * 256, m0 / 128 + (int)rank, bar);
           pair_load_box_2d(st + 2 * kXTile + kXScale, &wsmap, kb * 256, n0 / 128, bar);
           if (++s == kQStages) { s = 0; phase ^= 1; }
@@ -152,7 +170,10 @@ mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant
       const Desc xc(tma::desc_sw128(sm, 16, 1024)), wc(tma::desc_sw128(sm + kXTile, 16, 1024));
       const Desc xs(umma::smem_desc(sm + 2 * kXTile, 0, 128)), ws(umma::smem_desc(sm + 2 * kXTile + kXScale, 0, 128));
       int s = 0, phase = 0, local = 0;
-      for (int i = pair; i < tiles && !gave_up; i += pairs, ++local) {
+      for (int i = pair; i < units && !gave_up; i += pairs, ++local) {
+        int m0, n0, from, width;
+        unit_at(i, m0, n0, from, width);
+        const uint32_t idesc = idesc_mx4(256, width);
         const uint32_t acc = tm + (local & 1) * (256 - kQShared);
         if (local >= 1) wait(handed, (local - 1) & 1);                     // the other accumulator's shared columns, and all of this one, have been read
         for (int kb = 0; kb < kb_n; ++kb) {
@@ -163,7 +184,7 @@ mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant
           const int steps = P.K / 64 - kb * 4;
           if (one) {
             issue_scales<2, 2>(cols, xs, off, ws, off, steps);
-            issue_products<2, 2>(acc, xc, off, wc, off, cols, 0, idesc_mx4(256, 256), steps, kb == 0);
+            issue_products<2, 2>(acc, xc, off, wc, off, cols, from / 32, idesc, steps, kb == 0);
             umma::pair_commit(&empty[s]);                                         // the stage is free in both CTAs once these products have read it
             if (kb == kb_n - 1) umma::pair_commit(&accFull[local & 1]);
           }
@@ -175,9 +196,10 @@ mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant
     // ---------------------------------------------------------------- epilogue: four warps to each quarter of the lanes
     const int q = w & 3, h = (w - 2) >> 2;
     int local = 0;
-    for (int i = pair; i < tiles; i += pairs, ++local) {
-      int m0, n0;
-      tile_at(i, m0, n0);
+    for (int i = pair; i < units; i += pairs, ++local) {
+      int m0, n0, from, width;
+      unit_at(i, m0, n0, from, width);
+      n0 += from;
       const int odd = local & 1;
       if (l == 0) wait(&accFull[odd], (local >> 1) & 1);
       __syncwarp();
@@ -195,7 +217,7 @@ mx4_gemm_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant
           __syncwarp();
           if (l == 0) umma::pair_arrive_relaxed(umma::cluster_addr(handed, 0));
         }
-        if (live > 0 && n0 + 32 * c < P.N) store_columns(P, sm + kQTurn + (w - 2) * kTurnBytes, row0, n0 + 32 * c, v, live);
+        if (live > 0 && 32 * c < width && n0 + 32 * c < P.N) store_columns(P, sm + kQTurn + (w - 2) * kTurnBytes, row0, n0 + 32 * c, v, live);
       }
     }
   }
@@ -419,6 +441,25 @@ static cr_status mx4_split_launch(const ProjParams& P, const cr_mx4* x, const cr
   CR_LAUNCH_CHECK("mx4_gemm_split_kernel");
   return CR_OK;
 }
+
+template <int PARTS>
+static cr_status mx4_pair_launch(const ProjParams& P, const cr_mx4* x, const cr_mx4* w, long long tiles, int pairs, cudaStream_t stream) {
+  static PerDeviceOnce configured;
+  if (cr_status st = once_per_device(configured, [] {
+        CR_CUDA(cudaFuncSetAttribute(mx4_gemm_pair_kernel<PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kQSmem));
+        return CR_OK;
+      })) return st;
+  const long long whole = tiles / pairs * pairs, units = whole + (tiles - whole) * PARTS;
+  CUtensorMap xmap, wmap, cmap, xsmap, wsmap;
+  if (cr_status st = map_mx4(&xmap, &xsmap, x, 128, 1)) return st;
+  if (cr_status st = map_mx4(&wmap, &wsmap, w, 128, 2)) return st;
+  if (PARTS == 1) cmap = wmap;
+  else if (cr_status st = map_mx4(&cmap, &wsmap, w, 128 / PARTS, 2)) return st;
+  CR_CUDA(launch_pdl(mx4_gemm_pair_kernel<PARTS>, dim3(2 * (unsigned)(units < pairs ? units : pairs)), dim3(kQThreads), kQSmem, stream, P, xmap, wmap, cmap, xsmap,
+                     wsmap, (int)whole));
+  CR_LAUNCH_CHECK("mx4_gemm_pair_kernel");
+  return CR_OK;
+}
 }  // namespace cr
 
 extern "C" cr_status cr_mx4_gemm(const cr_mx4* x, const cr_mx4* w, const cr_proj_out* outs, int n_outs, void* stream_) {
@@ -436,17 +477,9 @@ extern "C" cr_status cr_mx4_gemm(const cr_mx4* x, const cr_mx4* w, const cr_proj
   if (shape.tn == 64) return mx4_split_launch<64>(P, x, w, shape.splits, stream);
   if (shape.tn == 128) return mx4_split_launch<128>(P, x, w, shape.splits, stream);
   if (shape.tn == 256) return mx4_split_launch<256>(P, x, w, shape.splits, stream);
-  static PerDeviceOnce configured;
-  if (cr_status st = once_per_device(configured, [] {
-        CR_CUDA(cudaFuncSetAttribute(mx4_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kQSmem));
-        return CR_OK;
-      })) return st;
-  CUtensorMap xmap, wmap, xsmap, wsmap;
-  if (cr_status st = map_mx4(&xmap, &xsmap, x, 128, 1)) return st;
-  if (cr_status st = map_mx4(&wmap, &wsmap, w, 128, 2)) return st;
   const long long tiles = (long long)((P.R + 255) / 256) * ((P.N + 255) / 256);
-  const int pairs = sm_count() / 2;
-  CR_CUDA(launch_pdl(mx4_gemm_pair_kernel, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), dim3(kQThreads), kQSmem, stream, P, xmap, wmap, xsmap, wsmap));
-  CR_LAUNCH_CHECK("mx4_gemm_pair_kernel");
-  return CR_OK;
+  const int pairs = sm_count() / 2, parts = pair_parts(tiles % pairs, pairs);
+  if (parts == 4) return mx4_pair_launch<4>(P, x, w, tiles, pairs, stream);
+  if (parts == 2) return mx4_pair_launch<2>(P, x, w, tiles, pairs, stream);
+  return mx4_pair_launch<1>(P, x, w, tiles, pairs, stream);
 }

@@ -174,6 +174,8 @@ def test_scale_bytes_of_no_row_are_left():
     (257, 512, [544], [True]),
     (2100, 1088, [2080, 288], [False, True]),                    # several waves of tiles, ragged both ways
     (5000, 128, [4128], [True]),                                 # more tiles than CTAs, short K
+    (2040, 320, [9792, 32], [True, False]),                      # the last wave's few tiles are cut into four
+    (2000, 192, [5536, 96], [False, True]),                      # and into two
 ])
 def test_product_of_two_4_bit_matrices(R, K, widths, f32):
     L = layers()
