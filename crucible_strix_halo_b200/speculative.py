@@ -30,7 +30,7 @@ class Head:
     w: layers.Mx4 [vocabulary, inner].  repetition, frequency, presence, bias [vocabulary]: as in layers.logits_choose, over all
     tokens of the stream, prompt included.  allowed: called with the stream's tokens and the drafts of a pass, gives the grammar's
     words for its 1 + len(drafts) rows (int32, [rows, ceil(vocabulary / 32)] or one row for all), or None where everything is
-    allowed."""
+    allowed.  Words that allow no token are a ValueError, behind which the stream is to be closed: the pass has run."""
 
     def __init__(self, w, repetition=1.0, frequency=0.0, presence=0.0, bias=None, allowed=None, rows=capi.MAX_STEP_ROWS):
         self.w, self.bias, self.allowed = w, bias, allowed

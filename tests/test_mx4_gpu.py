@@ -324,6 +324,48 @@ def test_a_row_that_is_not_finite_is_nan_and_leaves_the_others(value):
     check_product(x[keep].double().cpu(), values64(w), [y[keep]], 128)
 
 
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+@pytest.mark.parametrize("R", [13, 24, 60])
+def test_many_rows_of_which_one_is_not_finite(R, value):
+    L = layers()
+    x, w = torch.randn(R, 192, device="cuda").bfloat16(), random_mx4(288, 192, 2)
+    x[R - 2, 190] = value
+    y = torch.empty(R, 288, device="cuda")
+    L.mx4_rows(x, w, [y])
+    assert y[R - 2].isnan().all()
+    keep = [r for r in range(R) if r != R - 2]
+    check_product(x[keep].double().cpu(), values64(w), [y[keep]], 192)
+
+
+def test_many_rows_captured_and_beside_another_stream():
+    """24 rows at a time, the weights made by the call before: replayed with new rows and weights, another stream's calls in between."""
+    L = layers()
+    R, K, N = 24, 320, 9632
+    x, plain = torch.zeros(R, K, device="cuda", dtype=torch.bfloat16), torch.zeros(N, K, device="cuda")
+    w, y = L.Mx4.empty(N, K), torch.empty(R, N, device="cuda")
+    other, side = random_mx4(N, K, 8), torch.cuda.Stream()
+    xo = torch.randn(R, K, device="cuda")
+    want = torch.empty(R, N, device="cuda")
+    L.mx4_rows(xo, other, [want])
+    L.mx4_rows(x, L.mx4_quant(plain, out=w), [y])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(2):
+            L.mx4_rows(x, L.mx4_quant(plain, out=w), [y])
+    for seed in (1, 2):
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        x.copy_(torch.randn(R, K, device="cuda", generator=gen))
+        plain.copy_(torch.randn(N, K, device="cuda", generator=gen))
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(side):
+            yo = torch.empty(R, N, device="cuda")
+            L.mx4_rows(xo, other, [yo])
+        torch.cuda.synchronize()
+        check_product(x.double().cpu(), values64(w), [y], K)
+        assert torch.equal(yo, want)
+
+
 @pytest.mark.parametrize("call", ["gemm", "rows"])
 @pytest.mark.parametrize("R", [3, 130, 700])
 def test_outputs_at_a_pitch_leave_what_is_beside_them(call, R):
