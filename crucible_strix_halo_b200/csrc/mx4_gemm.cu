@@ -10,7 +10,8 @@
 // memory before they are stored 381, sixteen epilogue warps instead of eight 361: 4.6 PFLOP/s, 0.69 of four times the measured bf16
 // rate.  What bounds it now is the power cap: block after block of calls runs at 1.3 GHz and takes 416 us (the same products without
 // stores 332 us at 1.57 GHz); short K the stores (16,384 x 64 x 12,800: 5.1 TB/s).  Taken back: two whole accumulators on 256 x 192
-// tiles (384 us: more bytes a product), stores by the copy engine (387), waits that spin (K = 6,144: 103 -> 109 us).
+// tiles (384 us: more bytes a product), stores by the copy engine (387), stores of 32 bytes a lane from
+// registers (16,384 x 512 x 9,856, fp32: 125 -> 134), waits that spin (K = 6,144: 103 -> 109 us).
 // The few tiles of a last wave are cut into PARTS = 2 or 4, of 128 or 64 columns: 2,048 x 2,048 x 9,856 (312 tiles for 74 pairs) 28.8 -> 27.7 us,
 // 2,500 x 512 x 6,144 (240) 19.6 -> 17.7, 8,192 x 2,048 x 2,048 (256) 21.4 -> 20.6.
 //

@@ -22,6 +22,9 @@
 // digits' codes, which come from L2 once for 256 rows of W and not for 128.  At 131,072 x 2,048, against one CTA: 16 rows 30.9 and 32.8 us,
 // 20 rows 33.7 and 47.9, 24 rows 35.3 and 52.9, 72 rows (three passes) 79.6 and 131.7.
 //
+// Taken back: X's digits kept in shared memory beside a shorter ring (13 rows 30.3 -> 31.7 us); a digits kernel that lets this one in
+// before it waits, so that both start sooner and the weights are asked for later (4 rows 29.5 -> 31.4).
+//
 // What bounds it: W at 131,072 x 2,048 is 142.6 MB, 21.8 us at the copy bandwidth and 22.6 us for the same copies without products.  One row
 // takes 26.3 us, 9 rows 30.5, 13 rows 30.1 (4.9 TB/s): the launches, the first stage's and the last tile's latency, 4 to 7 us.  The
 // copying thread's divisions had cost 4 us; one accumulator for 11 to 19 rows 13 us, since the epilogue stands between two tiles then.
