@@ -29,6 +29,9 @@
 // takes 26.3 us, 9 rows 30.5, 13 rows 30.1 (4.9 TB/s): the launches, the first stage's and the last tile's latency, 4 to 7 us.  The
 // copying thread's divisions had cost 4 us; one accumulator for 11 to 19 rows 13 us, since the epilogue stands between two tiles then.
 // Calls over few weights are latencies: 1 x 64 x 32 3.6 us.
+//
+// Every wait is bounded (bit 6 of the device status word), and the bound is the kernel's own time: under a programmatic launch the kernel
+// ahead may run for as long as it likes, so every role waits for its end before its first bounded wait.
 #include <cooperative_groups.h>
 #include "mx4_mma.cuh"
 
@@ -210,6 +213,7 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
     const Desc ws(umma::smem_desc(sm + kXTile, 0, 128)), xs(umma::smem_desc(OWN ? own_scales : sm + kXTile + kXScale, 0, 128));
     const uint32_t idesc = idesc_mx4(kXM, S.cols), scales = tm + accs * acc_cols;
     int s = 0, phase = 0, local = 0;
+    pdl_wait();
     if constexpr (OWN) wait(ready, 0);
     for (int u = first; u < units && !gave_up; u += step, ++local) {
       const int a = accs == 2 ? local & 1 : 0, use = accs == 2 ? local >> 1 : local;
@@ -236,10 +240,10 @@ mx4_rows_kernel(const __grid_constant__ ProjParams P, const __grid_constant__ Ro
       }
     }
   } else {
+    pdl_wait();
     if constexpr (OWN) {
       // Eight elements a thread, in the places that a 128-byte-swizzled copy would give them: the 16-byte chunk of a row changes
       // places with its number xor the row's.
-      pdl_wait();
       const int D = digits_of(FROM), eights = kb_n * (kXK / 8), k0 = kb0 * kXK;
       for (int i = t - 64; i < S.pass_rows * eights; i += 256) {
         const int r = i / eights, e = i - r * eights, kb = e / 32, word = e % 32, b = word / 4;     // b: block of the stage
@@ -407,6 +411,7 @@ mx4_rows_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant
       const Desc ws(umma::smem_desc(sm + kXTile + xcodes, 0, 128)), xs(umma::smem_desc(sm + kXTile + xcodes + kXScale, 0, 128));
       const uint32_t idesc = idesc_mx4(256, S.cols), scales = tm + pair_scale_column(S.cols);
       int s = 0, phase = 0, local = 0;
+      pdl_wait();
       for (int u = first; u < units && !gave_up; u += step, ++local) {
         const int odd = local & 1;
         const uint32_t acc = tm + odd * pair_acc_step(S.cols);
@@ -437,6 +442,7 @@ mx4_rows_pair_kernel(const __grid_constant__ ProjParams P, const __grid_constant
     static_assert(GROUP * D <= 64 && 2 * GROUP == HALF, "");
     const int q = w & 3, h = (w - 2) >> 2;
     int local = 0;
+    pdl_wait();
     for (int u = first; u < units; u += step, ++local) {
       const int odd = local & 1, n0 = u / S.passes * 256 + 128 * (int)rank + 32 * q;
       const int r0 = u % S.passes * S.pass_rows + h * HALF, live = min(HALF, min(S.pass_rows - h * HALF, P.R - r0));   // rows of this half

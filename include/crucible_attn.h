@@ -484,7 +484,7 @@ cr_status cr_debug_umma_kv_step(const uint16_t* k_cache, const uint16_t* v_cache
 /* Test hook for the bounded waits: one CTA waits up to max_us microseconds on an mbarrier that nothing will ever
  * complete (no copy, no tensor-core work pending), then sets *status (device int) to 1, raises bit 3 of the device
  * status word and returns normally.  Shows that a wait that runs out ends the kernel and leaves the context
- * usable.  max_us in 1..100000.  No counterpart in the reference. */
+ * usable, and holds up the kernels behind it for longer than their own waits last.  max_us in 1..3000000.  No counterpart in the reference. */
 cr_status cr_debug_wait_timeout(int* status, unsigned max_us, void* stream);
 
 #ifdef __cplusplus
