@@ -315,7 +315,8 @@ PyObject* proj_gemm(PyObject*, PyObject* args) {     // (x, w, outs)
 }
 
 // ---- 4-bit projections and the choice of a token --------------------------------------------------------------------
-// These take tensors of several types and strides, so they look at what they are given.
+// These take tensors of several types and strides, so they look at what they are given.  An entry point that the library may lack is
+// looked up first, with the interpreter lock: its absence is an exception.
 [[noreturn]] void refuse(PyObject* type, const char* fmt, const char* what) { PyErr_Format(type, fmt, what); throw Error(); }
 template <typename F>
 F* present(F* f) {
@@ -385,6 +386,7 @@ std::vector<cr_proj_out> projections(PyObject* outs, int64_t rows) {
 
 PyObject* mx4_quant(PyObject*, PyObject* args) {     // (x, to, or the class of a new matrix)
   return guarded([&]() -> PyObject* {
+    auto* const entry = present(cr_mx4_quant);
     PyObject *x, *to;
     if (!PyArg_ParseTuple(args, "OO", &x, &to)) throw Error();
     const at::Tensor& xt = here(x, "x");
@@ -413,7 +415,7 @@ PyObject* mx4_quant(PyObject*, PyObject* args) {     // (x, to, or the class of 
     Ref held(out);
     const void* const xp = xt.data_ptr();
     void* const st = stream();
-    check(unlocked([&] { return present(cr_mx4_quant)(xp, type, ld, &m, st); }));
+    check(unlocked([&] { return entry(xp, type, ld, &m, st); }));
     Py_INCREF(out);
     return out;
   });
@@ -421,6 +423,7 @@ PyObject* mx4_quant(PyObject*, PyObject* args) {     // (x, to, or the class of 
 
 PyObject* mx4_dequant(PyObject*, PyObject* args) {   // (m, out, or the type of new rows)
   return guarded([&]() -> PyObject* {
+    auto* const entry = present(cr_mx4_dequant);
     PyObject *from, *to;
     if (!PyArg_ParseTuple(args, "OO", &from, &to)) throw Error();
     const cr_mx4 m = mx4(from, "the 4-bit matrix");
@@ -431,7 +434,7 @@ PyObject* mx4_dequant(PyObject*, PyObject* args) {   // (m, out, or the type of 
     const int64_t ld = pitch(t, "out");
     if (t.size(0) != m.rows || t.size(1) != m.inner) refuse(PyExc_ValueError, "%s has another shape than the 4-bit matrix", "out");
     void *const p = t.data_ptr(), *const st = stream();
-    check(unlocked([&] { return present(cr_mx4_dequant)(&m, p, type, ld, st); }));
+    check(unlocked([&] { return entry(&m, p, type, ld, st); }));
     Py_INCREF(out.p);
     return out.p;
   });
@@ -439,12 +442,13 @@ PyObject* mx4_dequant(PyObject*, PyObject* args) {   // (m, out, or the type of 
 
 PyObject* mx4_gemm(PyObject*, PyObject* args) {      // (x, w, outs)
   return guarded([&]() -> PyObject* {
+    auto* const entry = present(cr_mx4_gemm);
     PyObject *x, *w, *outs;
     if (!PyArg_ParseTuple(args, "OOO", &x, &w, &outs)) throw Error();
     const cr_mx4 xm = mx4(x, "x"), wm = mx4(w, "w");
     const std::vector<cr_proj_out> o = projections(outs, xm.rows);
     void* const st = stream();
-    check(unlocked([&] { return present(cr_mx4_gemm)(&xm, &wm, o.data(), (int)o.size(), st); }));
+    check(unlocked([&] { return entry(&xm, &wm, o.data(), (int)o.size(), st); }));
     Py_INCREF(outs);
     return outs;
   });
@@ -452,6 +456,8 @@ PyObject* mx4_gemm(PyObject*, PyObject* args) {      // (x, w, outs)
 
 PyObject* mx4_rows(PyObject*, PyObject* args) {      // (x, w, outs)
   return guarded([&]() -> PyObject* {
+    auto* const entry = present(cr_mx4_rows);
+    auto* const workspace_bytes = present(cr_mx4_rows_workspace_bytes);
     PyObject *x, *w, *outs;
     if (!PyArg_ParseTuple(args, "OOO", &x, &w, &outs)) throw Error();
     const at::Tensor& xt = here(x, "x");
@@ -461,12 +467,12 @@ PyObject* mx4_rows(PyObject*, PyObject* args) {      // (x, w, outs)
     if (xt.size(1) != wm.inner) refuse(PyExc_ValueError, "%s has another number of elements in a row than w", "x");
     const std::vector<cr_proj_out> o = projections(outs, xt.size(0));
     const int R = count(xt.size(0), "x");
-    const size_t bytes = present(cr_mx4_rows_workspace_bytes)(R, wm.inner);
+    const size_t bytes = workspace_bytes(R, wm.inner);
     const at::Tensor ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(xt.device()));   // of the current stream
     void* const wsp = ws.data_ptr();
     const void* const xp = xt.data_ptr();
     void* const st = stream();
-    check(unlocked([&] { return present(cr_mx4_rows)(xp, type, ld, R, &wm, wsp, bytes, o.data(), (int)o.size(), st); }));
+    check(unlocked([&] { return entry(xp, type, ld, R, &wm, wsp, bytes, o.data(), (int)o.size(), st); }));
     Py_INCREF(outs);
     return outs;
   });
@@ -486,6 +492,7 @@ PyObject* item_or_none(PyObject* dict, PyObject* name) {
 }
 PyObject* logits_choose(PyObject*, PyObject* args) { // (spans, outs or None) -> choices
   return guarded([&]() -> PyObject* {
+    auto* const entry = present(cr_logits_choose);
     PyObject *spans, *given;
     if (!PyArg_ParseTuple(args, "OO", &spans, &given)) throw Error();
     Ref list(PySequence_Fast(spans, "spans must be a sequence"));
@@ -534,7 +541,7 @@ PyObject* logits_choose(PyObject*, PyObject* args) { // (spans, outs or None) ->
       a[i].choice = flat<int>(o, at::kInt, R, "a choice", dev);
     }
     void* const st = stream();
-    check(unlocked([&] { return present(cr_logits_choose)(a.data(), (int)n, st); }));
+    check(unlocked([&] { return entry(a.data(), (int)n, st); }));
     Py_INCREF(outs.p);
     return outs.p;
   });
@@ -542,6 +549,7 @@ PyObject* logits_choose(PyObject*, PyObject* args) { // (spans, outs or None) ->
 
 PyObject* token_count(PyObject*, PyObject* args) {   // (counts, tokens, delta)
   return guarded([&]() -> PyObject* {
+    auto* const entry = present(cr_token_count);
     PyObject *counts, *tokens;
     int delta;
     if (!PyArg_ParseTuple(args, "OOi", &counts, &tokens, &delta)) throw Error();
@@ -549,7 +557,7 @@ PyObject* token_count(PyObject*, PyObject* args) {   // (counts, tokens, delta)
     const int* const t = flat<int>(tokens, at::kInt, 0, "tokens");
     const int V = count(tensor(counts).numel(), "counts"), n = count(tensor(tokens).numel(), "tokens");
     void* const st = stream();
-    check(unlocked([&] { return present(cr_token_count)(t, n, delta, c, V, st); }));
+    check(unlocked([&] { return entry(t, n, delta, c, V, st); }));
     Py_INCREF(counts);
     return counts;
   });
