@@ -19,6 +19,8 @@ glue protocol:
     mtp_rows(tokens, stacks)         -> (q, k, v, idx) of the draft layer for rows (token p+1, stack of position p)
     draft(mtp_out_row, position)     -> one token id
 """
+import math
+
 import torch
 
 from . import capi, layers
@@ -27,18 +29,29 @@ from . import capi, layers
 class Head:
     """The head of one stream and its sampler's greedy part: output rows [R, inner] -> tokens.
 
-    w: layers.Mx4 [vocabulary, inner].  repetition, frequency, presence, bias [vocabulary]: as in layers.logits_choose, over all
-    tokens of the stream, prompt included.  allowed: called with the stream's tokens and the drafts of a pass, gives the grammar's
-    words for its 1 + len(drafts) rows (int32, [rows, ceil(vocabulary / 32)] or one row for all), or None where everything is
-    allowed.  Words that allow no token are a ValueError, behind which the stream is to be closed: the pass has run."""
+    w: layers.Mx4 [rows, inner], a multiple of 32 rows: the first `vocabulary` of them (all, where it is not given) are the tokens',
+    those behind (zeros, for instance) are never chosen.  repetition, frequency, presence, bias (float32, [vocabulary]): as in
+    layers.logits_choose, over all tokens of the stream, prompt included.  allowed: called with the stream's tokens and the drafts of
+    a pass, gives the grammar's words for its 1 + len(drafts) rows (int32, [rows, ceil(vocabulary / 32)] or one row for all), or None
+    where everything is allowed.  Words that allow no token are a ValueError, behind which the stream is to be closed: the pass has
+    run.  What every pass would refuse is a ValueError here."""
 
-    def __init__(self, w, repetition=1.0, frequency=0.0, presence=0.0, bias=None, allowed=None, rows=capi.MAX_STEP_ROWS):
-        self.w, self.bias, self.allowed = w, bias, allowed
+    def __init__(self, w, repetition=1.0, frequency=0.0, presence=0.0, bias=None, allowed=None, rows=capi.MAX_STEP_ROWS, vocabulary=None):
+        vocabulary = w.rows if vocabulary is None else vocabulary
+        if w.rows % 32:
+            raise ValueError("the head's matrix has %d rows: it needs a multiple of 32, the tokens' first (vocabulary says how many)" % w.rows)
+        if not 1 <= vocabulary <= w.rows:
+            raise ValueError("a vocabulary of %d tokens, of a matrix of %d rows" % (vocabulary, w.rows))
+        if not (0 < repetition < math.inf and abs(frequency) < math.inf and abs(presence) < math.inf):
+            raise ValueError("penalties must be finite, the repetition penalty positive")
+        if bias is not None and not (bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() >= vocabulary):
+            raise ValueError("the bias must be float32, contiguous, and hold %d numbers" % vocabulary)
+        self.w, self.bias, self.allowed, self.vocabulary = w, bias, allowed, vocabulary
         self.penalties = dict(repetition=repetition, frequency=frequency, presence=presence)
         device = w.codes.device
         self.logits = torch.empty(rows, w.rows, device=device)
         self.choice = torch.empty(rows, device=device, dtype=torch.int32)
-        self.counts = torch.zeros(w.rows, device=device, dtype=torch.int32)
+        self.counts = torch.zeros(vocabulary, device=device, dtype=torch.int32)
 
     def accept(self, tokens):
         """Tokens that the stream has taken in: from now on they count."""
@@ -49,7 +62,7 @@ class Head:
         R = len(drafts) + 1
         logits, choice = self.logits[:R], self.choice[:R]
         layers.mx4_rows(out, self.w, [logits])
-        span = dict(logits=logits, counts=self.counts, bias=self.bias, mask=self.allowed(tokens, drafts) if self.allowed else None, **self.penalties)
+        span = dict(logits=logits[:, :self.vocabulary], counts=self.counts, bias=self.bias, mask=self.allowed(tokens, drafts) if self.allowed else None, **self.penalties)
         if drafts:
             span["drafts"] = torch.tensor(drafts, device=choice.device, dtype=torch.int32)
         ids = layers.logits_choose([span], [choice])[0].tolist()
