@@ -34,7 +34,7 @@ class Head:
     layers.logits_choose, over all tokens of the stream, prompt included.  allowed: called with the stream's tokens and the drafts of
     a pass, gives the grammar's words for its 1 + len(drafts) rows (int32, [rows, ceil(vocabulary / 32)] or one row for all), or None
     where everything is allowed.  Words that allow no token are a ValueError, behind which the stream is to be closed: the pass has
-    run.  What every pass would refuse is a ValueError here."""
+    run.  rows: of the longest pass, the stream's span at least.  What every pass would refuse is a ValueError here."""
 
     def __init__(self, w, repetition=1.0, frequency=0.0, presence=0.0, bias=None, allowed=None, rows=capi.MAX_STEP_ROWS, vocabulary=None):
         vocabulary = w.rows if vocabulary is None else vocabulary
@@ -81,6 +81,8 @@ class SpecStream:
 
     def __init__(self, g, gdn_weights, qsa_weights, mtp_weights, glue, ctx, mtp_rows=0, span=9, head=None):
         assert 2 <= span <= capi.MAX_STEP_ROWS
+        if head is not None and len(head.choice) < span:
+            raise ValueError("a head of %d rows for spans of %d" % (len(head.choice), span))
         self.g, self.glue, self.span, self.head = g, glue, span, head
         self.gw, self.qw, self.mw = gdn_weights, qsa_weights, mtp_weights
         self.gs = [layers.GdnSession(g, pend_rows=16 if span > 8 else 8) for _ in gdn_weights]

@@ -1,4 +1,4 @@
-"""What speculative.Head refuses before a pass has run.  No GPU is needed: nothing is computed."""
+"""What speculative.Head, and a stream that is given one, refuse before a pass has run.  No GPU is needed: nothing is computed."""
 import math
 
 import pytest
@@ -33,3 +33,8 @@ def test_a_vocabulary_smaller_than_the_matrix(spec):
     head = spec.Head(_matrix(1024), vocabulary=1003, bias=torch.zeros(1003))
     assert head.counts.shape == (1003,) and head.logits.shape == (13, 1024)
     assert spec.Head(_matrix(1024)).counts.shape == (1024,)
+
+
+def test_a_head_of_fewer_rows_than_a_span(spec):
+    with pytest.raises(ValueError, match="rows"):
+        spec.SpecStream(None, [], None, None, None, 64, span=9, head=spec.Head(_matrix(64), rows=8))
