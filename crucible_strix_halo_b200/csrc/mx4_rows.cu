@@ -8,7 +8,8 @@
 // with 2^E above the largest of x's block of 32.  A digit is an e2m1 number and its weight an e8m0 scale, so that the digits of a row
 // are rows of a 4-bit matrix.  Ten of them for bf16 and fp16 rows, twelve for fp32 rows: an element is off by at most 2^(E - 30) or
 // 2^(E - 36), and exact where it has no bits below twice that, so that a channel a thousand times the others' size takes
-// nothing from them.  The sums of an output's digits, each in fp32, are added from the smallest up.  The order of all sums depends on N
+// nothing from them.  No weight is below 2^-127, the smallest scale: where that comes first an element is off by at most 2^-128.
+// The sums of an output's digits, each in fp32, are added from the smallest up.  The order of all sums depends on N
 // and K alone: a row has the same bits in every call.
 //
 // mx4_rows_kernel: 128 rows of W are the M side, up to 256 digit rows the N side; persistent over W (up to 128 digit rows), or one tile
@@ -65,7 +66,8 @@ __device__ __forceinline__ void make_digits(float (&v)[8], unsigned quad, F&& pu
   for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
   top = max(top, __shfl_xor_sync(quad, top, 1));
   top = max(top, __shfl_xor_sync(quad, top, 2));
-  const int field = max((int)(top >> 23), 1);                      // 2^(field - 126) is above every element; 255: not finite
+  int field = max((int)(top >> 23), 1);                            // 2^(field - 126) is above every element; 255: not finite
+  if (field <= 3 * D - 2) field = (field + 1) / 3 * 3 + 1;         // where the weights go below 2^-127, the last one is 2^-127 itself
   const float up = __uint_as_float((uint32_t)(field == 255 ? 1 : 255 - field) << 23);
   f2 x[4];
 #pragma unroll
@@ -82,7 +84,7 @@ __device__ __forceinline__ void make_digits(float (&v)[8], unsigned quad, F&& pu
       d[2 * k] = f.x;
       d[2 * k + 1] = f.y;
     }
-    const int scale = field - 1 - 3 * j;                           // below 0: what is left lies under 2^-127
+    const int scale = field - 1 - 3 * j;                           // below 0: what is left, 2^-128 at most, is left out
     put(j, field == 255 || scale < 0 ? 0u : pack_e2m1(d, 1.f), field == 255 ? 255 : (uint8_t)max(scale, 0));
   }
 }

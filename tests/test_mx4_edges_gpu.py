@@ -32,3 +32,51 @@ def test_the_time_of_the_kernel_ahead_is_not_the_products_own():
     check_product(x[:1].double().cpu(), values64(w), [one], 256)
     check_product(x.double().cpu(), values64(w), [many], 256)
     check_product(values64(xq), values64(w), [y], 256)
+
+
+def _ones(K, byte):
+    """K x K, the identity times 2^(byte - 127)."""
+    w = layers().Mx4.empty(K, K)
+    w.codes.zero_()
+    i = torch.arange(K, device="cuda")
+    w.codes[i, i // 2] = torch.where(i % 2 == 0, 2, 32).to(torch.uint8)       # code 2 is 1.0
+    w.scales.fill_(byte)
+    return w
+
+
+def _rows_of_sizes(exponents, K, dtype, seed):
+    """A row for each exponent: its largest element is in [2^e, 2^(e + 1)), the others are of that size and of every smaller one."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    e = torch.tensor(exponents, device="cuda", dtype=torch.float64)[:, None]
+    u = lambda: torch.rand(len(exponents), K, device="cuda", generator=gen, dtype=torch.float64)
+    down = torch.floor(40 * u() ** 2)
+    x = (1 + u()) * torch.exp2(e - down) * torch.where(u() < 0.5, -1.0, 1.0)
+    x[:, ::32] = torch.exp2(e)                                                # one of every block has the exponent, and is exact
+    x[:, 5] = (2 - 2.0 ** -7) * torch.exp2(e)[:, 0]                           # the largest of a 16-bit type with it
+    x = torch.where(x.abs() < torch.exp2(e + 1) * (1 - 2.0 ** -9), x, torch.exp2(e))
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("exponents,byte", [(range(-126, -84), 187), (range(-84, -60), 127), (range(100, 126), 100)])
+def test_every_element_is_as_near_as_the_header_says(exponents, byte, dtype):
+    """Products with the identity give the elements back, each with the error of its digits alone: what the digits hold of an element is a
+    multiple of the last one's weight or of the element's own last bit, so that their sums are exact but for the final one."""
+    L = layers()
+    K, exponents = 128, list(exponents)
+    x, w = _rows_of_sizes(exponents, K, dtype, 1), _ones(K, byte)
+    y = torch.empty(len(exponents), K, device="cuda")
+    L.mx4_rows(x, w, [y])
+    digits = 12 if dtype == torch.float32 else 10
+    e = torch.tensor(exponents, dtype=torch.float64)[:, None]
+    limit = torch.exp2(e + 1 - 3 * digits)
+    limit = limit.clamp(min=2.0 ** -128)
+    x64, got = x.double().cpu(), y.double().cpu() * 2.0 ** (127 - byte)
+    assert torch.isfinite(got).all()
+    # one rounding of the sum, and one where it lies under fp32's normal numbers
+    over = (got - x64).abs() - limit - 2.0 ** -24 * x64.abs() - 2.0 ** (-150 + 127 - byte)
+    assert over.max() <= 0, "row %d of exponent %d" % (int(over.amax(1).argmax()), exponents[int(over.amax(1).argmax())])
+    for r in range(0, len(exponents), 5):                                     # a row alone makes its digits itself
+        one = torch.empty(1, K, device="cuda")
+        L.mx4_rows(x[r:r + 1], w, [one])
+        assert torch.equal(one[0], y[r])
