@@ -8,9 +8,9 @@
 // with 2^E above the largest of x's block of 32.  A digit is an e2m1 number and its weight an e8m0 scale, so that the digits of a row
 // are rows of a 4-bit matrix.  Ten of them for bf16 and fp16 rows, twelve for fp32 rows: an element is off by at most 2^(E - 30) or
 // 2^(E - 36), and exact where it has no bits below twice that, so that a channel a thousand times the others' size takes
-// nothing from them.  No weight is below 2^-127, the smallest scale: where that comes first an element is off by at most 2^-128.
-// The sums of an output's digits, each in fp32, are added from the smallest up.  The order of all sums depends on N
-// and K alone: a row has the same bits in every call.
+// nothing from them.  No weight is below 2^-127, the smallest scale: where that comes first an element is off by at most 2^-128.  (E = 128,
+// the range's last octave: twice the bound.)  The sums of an output's digits, each in fp32, are added from the smallest up.  The order
+// of all sums depends on N and K alone: a row has the same bits in every call.
 //
 // mx4_rows_kernel: 128 rows of W are the M side, up to 256 digit rows the N side; persistent over W (up to 128 digit rows), or one tile
 // per cluster of CTAs that share K where there are few tiles.  With few elements of X for a CTA it makes their digits itself, into the tiles that the
@@ -68,23 +68,32 @@ __device__ __forceinline__ void make_digits(float (&v)[8], unsigned quad, F&& pu
   top = max(top, __shfl_xor_sync(quad, top, 2));
   int field = max((int)(top >> 23), 1);                            // 2^(field - 126) is above every element; 255: not finite
   if (field <= 3 * D - 2) field = (field + 1) / 3 * 3 + 1;         // where the weights go below 2^-127, the last one is 2^-127 itself
+  // In the range's last octave a first digit of 4 would stand for 2^128, with sums that overflow where the product does not: it is
+  // held to 3, and the next digit's weight is a quarter of its.
+  const bool last_octave = field == 254;
   const float up = __uint_as_float((uint32_t)(field == 255 ? 1 : 255 - field) << 23);
   f2 x[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) x[k] = mul2(pack2(v[2 * k], v[2 * k + 1]), pack2(up, up));       // below 4
   const f2 whole = pack2(12582912.f, 12582912.f), back = pack2(-12582912.f, -12582912.f), minus = pack2(-1.f, -1.f), eight = pack2(8.f, 8.f);
+  const f2 second = last_octave ? pack2(4.f, 4.f) : eight;
 #pragma unroll
   for (int j = 0; j < D; ++j) {
     float d[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const f2 n = add2(add2(x[k], whole), back);                  // 1.5 2^23 leaves no room behind the point: the nearest whole number
-      x[k] = mul2(fma2(n, minus, x[k]), eight);
-      const float2 f = unpack2(n);
+      f2 n = add2(add2(x[k], whole), back);                        // 1.5 2^23 leaves no room behind the point: the nearest whole number
+      float2 f = unpack2(n);
+      if (j == 0) {
+        const float most = last_octave ? 3.f : 4.f;
+        f = make_float2(fminf(fmaxf(f.x, -most), most), fminf(fmaxf(f.y, -most), most));
+        n = pack2(f.x, f.y);
+      }
+      x[k] = mul2(fma2(n, minus, x[k]), j == 0 ? second : eight);
       d[2 * k] = f.x;
       d[2 * k + 1] = f.y;
     }
-    const int scale = field - 1 - 3 * j;                           // below 0: what is left, 2^-128 at most, is left out
+    const int scale = field - 1 - 3 * j + (j > 0 && last_octave);  // below 0: what is left, 2^-128 at most, is left out
     put(j, field == 255 || scale < 0 ? 0u : pack_e2m1(d, 1.f), field == 255 ? 255 : (uint8_t)max(scale, 0));
   }
 }

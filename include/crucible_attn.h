@@ -394,8 +394,8 @@ cr_status cr_mx4_gemm(const cr_mx4* x, const cr_mx4* w, const cr_proj_out* outs,
 /* The same product with the rows of X as they are, [R][ld] of the given type (ld >= w->inner, any alignment of the type): the
  * projections of decode and verify rows, and the head, where the weights' bytes set the time.  Any R in 1..2^20 - 1 (R * w->inner
  * below 2^35, R * w->rows below 2^40); made for a few rows, each 24 of them (20 of fp32) read the weights once.  X enters as 4-bit
- * digits: an element is off by at most 2^-30 (fp32: 2^-36) of the power of two above the largest of its block of 32, or by
- * 2^-128 where that is more.  The bits of a row do not depend on the other rows of the call nor on their number.  A row that holds
+ * digits: an element is off by at most 2^-30 (fp32: 2^-36) of the power of two above the largest of its block of 32 (twice that where
+ * the largest is 2^127 or more), or by 2^-128 where that is more.  The bits of a row do not depend on the other rows of the call nor on their number.  A row that holds
  * an infinity or a NaN gives NaN.  `workspace`: cr_mx4_rows_workspace_bytes(R, w->inner) bytes, 16-byte aligned, of this call alone
  * until it has run.  Bit 6 of the device status word reports a bounded wait that gave up. */
 size_t cr_mx4_rows_workspace_bytes(int R, int inner);

@@ -58,7 +58,7 @@ def _rows_of_sizes(exponents, K, dtype, seed):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("exponents,byte", [(range(-126, -84), 187), (range(-84, -60), 127), (range(100, 126), 100)])
+@pytest.mark.parametrize("exponents,byte", [(range(-126, -84), 187), (range(-84, -60), 127), (range(100, 128), 127), (range(118, 128), 100)])
 def test_every_element_is_as_near_as_the_header_says(exponents, byte, dtype):
     """Products with the identity give the elements back, each with the error of its digits alone: what the digits hold of an element is a
     multiple of the last one's weight or of the element's own last bit, so that their sums are exact but for the final one."""
@@ -69,7 +69,7 @@ def test_every_element_is_as_near_as_the_header_says(exponents, byte, dtype):
     L.mx4_rows(x, w, [y])
     digits = 12 if dtype == torch.float32 else 10
     e = torch.tensor(exponents, dtype=torch.float64)[:, None]
-    limit = torch.exp2(e + 1 - 3 * digits)
+    limit = torch.exp2(e + 1 - 3 * digits) * torch.where(e == 127, 2, 1)
     limit = limit.clamp(min=2.0 ** -128)
     x64, got = x.double().cpu(), y.double().cpu() * 2.0 ** (127 - byte)
     assert torch.isfinite(got).all()
@@ -80,3 +80,15 @@ def test_every_element_is_as_near_as_the_header_says(exponents, byte, dtype):
         one = torch.empty(1, K, device="cuda")
         L.mx4_rows(x[r:r + 1], w, [one])
         assert torch.equal(one[0], y[r])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_types_largest_numbers(dtype):
+    """Products of the largest numbers with ones do not overflow, and have their bits."""
+    L = layers()
+    top = torch.finfo(dtype).max
+    x = torch.zeros(3, 64, device="cuda", dtype=dtype)
+    x[0, 3], x[1, 40], x[2, 63] = top, -top, top * 0.875
+    w, y = _ones(64, 127), torch.empty(3, 64, device="cuda")
+    L.mx4_rows(x, w, [y])
+    assert torch.equal(y, x.float())
