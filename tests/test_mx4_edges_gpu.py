@@ -92,3 +92,66 @@ def test_the_types_largest_numbers(dtype):
     w, y = _ones(64, 127), torch.empty(3, 64, device="cuda")
     L.mx4_rows(x, w, [y])
     assert torch.equal(y, x.float())
+
+
+def _scaled(m, byte):
+    """Gives block b of row r of a 4-bit matrix the scale byte[r, b]."""
+    r, b = torch.arange(m.rows, device="cuda")[:, None], torch.arange(m.inner // 32, device="cuda")[None]
+    m.scales[r // 128 * ((m.inner + 127) // 128) * 512 + b // 4 * 512 + r % 32 * 16 + r % 128 // 32 * 4 + b % 4] = byte.to(torch.uint8)
+
+
+def _launched(name, call):
+    """The kernels that `call` launches hold one of that name."""
+    from crucible_strix_halo_b200 import capi
+    stream = torch.cuda.current_stream().cuda_stream
+    capi.check(capi.lib.cr_profile_enable(1))
+    try:
+        capi.check(capi.lib.cr_profile_begin(stream))
+        call()
+        return name in capi.profile_collect()
+    finally:
+        capi.check(capi.lib.cr_profile_enable(0))
+
+
+@pytest.mark.parametrize("R,K,N,kernel", [
+    (4000, 1088, 4128, "mx4_gemm_pair_kernel"),                  # 16 x 17 tiles of 256 x 256: what is left of the last wave whole,
+    (2040, 1088, 9824, "mx4_gemm_pair_kernel"),                  # in four
+    (2000, 1088, 5632, "mx4_gemm_pair_kernel"),                  # and in two
+    (300, 1088, 2048, "mx4_gemm_split_kernel"),
+])
+def test_scales_that_differ_from_row_to_row_and_block_to_block(R, K, N, kernel):
+    """Scales from 0 to 254: those of a block are far from its neighbours' in X and as far the other way in W, and every row of X and of W
+    has an offset of its own, so that the products of an output are of one size, and another output's are of another."""
+    L = layers()
+    x, w = random_mx4(R, K, 1), random_mx4(N, K, 2)
+    b = torch.arange(K // 32, device="cuda")[None]
+    size = b * 97 % 34 * 7                                       # 0..231, all different
+    t, u = (torch.arange(n, device="cuda")[:, None] * 5 % 23 for n in (R, N))
+    _scaled(x, size + t)                                         # 0..253
+    _scaled(w, 254 - size - u)
+    y = torch.empty(R, N, device="cuda")
+    assert _launched(kernel, lambda: L.mx4_gemm(x, w, [y]))
+    check_product(values64(x), values64(w), [y], K)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("low", [0, 54])
+@pytest.mark.parametrize("R,N", [(1, 96), (9, 9632), (16, 9632), (24, 9632), (50, 9632)])
+def test_rows_with_weights_of_every_scale(R, N, low, dtype):
+    """Scales of W from 0 to 199 and from 54 to 253, elements of X as much larger or smaller."""
+    L = layers()
+    K = 1088
+    gen = torch.Generator(device="cuda").manual_seed(R)
+    w = random_mx4(N, K, 2)
+    b = torch.arange(K // 32, device="cuda")[None]
+    size = b * 97 % 34 * 53 // 10                                # 0..174
+    u = torch.arange(N, device="cuda")[:, None] * 5 % 26
+    _scaled(w, low + size + u)                                   # low..low + 199
+    e = (110 if low == 0 else 56) - size.double().repeat_interleave(32, 1)
+    x = ((1 + torch.rand(R, K, device="cuda", generator=gen, dtype=torch.float64)) * torch.exp2(e)).to(dtype)
+    x = torch.where(torch.rand(R, K, device="cuda", generator=gen) < 0.5, -x, x)
+    y = torch.empty(R, N, device="cuda")
+    L.mx4_rows(x, w, [y])
+    x64, w64 = x.double().cpu(), values64(w)
+    limit = K * 2.0 ** -24 * (x64.abs() @ w64.abs().t()) + 2.0 ** -128 * w64.abs().sum(1)
+    assert ((y.double().cpu() - x64 @ w64.t()).abs() <= limit).all()
