@@ -43,6 +43,7 @@ namespace cr {
 CR_DEFINE_STATUS_WORD(mx4_rows)
 
 constexpr int kDigitsMost = 12, kPassRows = 256;                 // digit rows of a pass over W
+constexpr int kRowsEnd = 1 << 20;                                // rows of X: fewer
 __host__ __device__ constexpr int digits_of(int dtype) { return dtype == CR_ROW_F32 ? 12 : 10; }
 // Digit rows come in halves of 128: so many rows of X fill one, twice as many make a pass.
 __host__ __device__ constexpr int half_rows(int digits) { return 128 / digits; }
@@ -556,7 +557,7 @@ static int rows_passes(int R, int digits) {
   return (R + most - 1) / most;
 }
 extern "C" size_t cr_mx4_rows_workspace_bytes(int R, int inner) {
-  if (R < 1 || inner < 1) return 0;
+  if (R < 1 || R >= cr::kRowsEnd || inner < 1) return 0;
   const int rows = rows_passes(R, cr::kDigitsMost) * cr::kPassRows;
   return cr_mx4_code_bytes(rows, inner) + cr_mx4_scale_bytes(rows, inner);
 }
@@ -565,7 +566,7 @@ extern "C" cr_status cr_mx4_rows(const void* x, cr_row_dtype dtype, long long ld
                                  const cr_proj_out* outs, int n_outs, void* stream_) {
   using namespace cr;
   if (cr_status s = check_mx4(w, "cr_mx4_rows", "W")) return s;
-  CR_REQUIRE(R >= 1 && R < (1 << 20), "cr_mx4_rows: R=%d rows", R);
+  CR_REQUIRE(R >= 1 && R < kRowsEnd, "cr_mx4_rows: R=%d rows", R);
   if (cr_status s = check_rows(x, dtype, ld, w->inner, "cr_mx4_rows")) return s;
   CR_REQUIRE((long long)R * w->inner < (1ll << 35) && (long long)R * w->rows < (1ll << 40), "cr_mx4_rows: %d rows of %d x %d are too many for a call", R, w->rows, w->inner);
   CR_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= cr_mx4_rows_workspace_bytes(R, w->inner),

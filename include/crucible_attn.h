@@ -397,7 +397,7 @@ cr_status cr_mx4_gemm(const cr_mx4* x, const cr_mx4* w, const cr_proj_out* outs,
  * digits: an element is off by at most 2^-30 (fp32: 2^-36) of the power of two above the largest of its block of 32 (twice that where
  * the largest is 2^127 or more), or by 2^-128 where that is more.  The bits of a row do not depend on the other rows of the call nor on their number.  A row that holds
  * an infinity or a NaN gives NaN.  `workspace`: cr_mx4_rows_workspace_bytes(R, w->inner) bytes, 16-byte aligned, of this call alone
- * until it has run.  Bit 6 of the device status word reports a bounded wait that gave up. */
+ * until it has run (0 for an R that no call takes).  Bit 6 of the device status word reports a bounded wait that gave up. */
 size_t cr_mx4_rows_workspace_bytes(int R, int inner);
 cr_status cr_mx4_rows(const void* x, cr_row_dtype dtype, long long ld, int R, const cr_mx4* w, void* workspace,
                       size_t workspace_bytes, const cr_proj_out* outs, int n_outs, void* stream);
