@@ -347,7 +347,7 @@ int64_t pitch(const at::Tensor& t, const char* what) {
   return t.stride(0);
 }
 int count(int64_t n, const char* what) {
-  if (n > INT32_MAX) refuse(PyExc_ValueError, "%s is too long", what);
+  if (n > INT32_MAX || n < 0) refuse(PyExc_ValueError, n < 0 ? "%s has a negative size" : "%s is too long", what);
   return (int)n;
 }
 // `n` elements of a type side by side.
@@ -360,8 +360,8 @@ T* flat(PyObject* o, at::ScalarType type, int64_t n, const char* what, int devic
 }
 cr_mx4 mx4(PyObject* o, const char* what) {
   cr_mx4 m{};
-  m.rows = (int)long_attr(o, s_rows);
-  m.inner = (int)long_attr(o, s_inner);
+  m.rows = count(long_attr(o, s_rows), what);
+  m.inner = count(long_attr(o, s_inner), what);
   if (m.rows < 1 || m.inner < 1 || m.inner % 2) refuse(PyExc_ValueError, "%s has no rows, or an odd number of elements in a row", what);
   Ref c(PyObject_GetAttr(o, s_codes)), s(PyObject_GetAttr(o, s_scales));
   m.codes = flat<uint8_t>(c, at::kByte, (int64_t)m.rows * m.inner / 2, what);
