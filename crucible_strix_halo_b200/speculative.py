@@ -34,7 +34,10 @@ class Head:
     layers.logits_choose, over all tokens of the stream, prompt included.  allowed: called with the stream's tokens and the drafts of
     a pass, gives the grammar's words for its 1 + len(drafts) rows (int32, [rows, ceil(vocabulary / 32)] or one row for all), or None
     where everything is allowed.  Words that allow no token are a ValueError, behind which the stream is to be closed: the pass has
-    run.  rows: of the longest pass, the stream's span at least.  What every pass would refuse is a ValueError here."""
+    run.  rows: of the longest pass, the stream's span at least.  What every pass would refuse is a ValueError here.
+
+    counts is no part of layers.checkpoint_spans: whoever restores a stream takes the tokens back that it no longer has, with
+    layers.token_count(head.counts, tokens, -1)."""
 
     def __init__(self, w, repetition=1.0, frequency=0.0, presence=0.0, bias=None, allowed=None, rows=capi.MAX_STEP_ROWS, vocabulary=None):
         vocabulary = w.rows if vocabulary is None else vocabulary

@@ -411,7 +411,8 @@ cr_status cr_mx4_rows(const void* x, cr_row_dtype dtype, long long ld, int R, co
  *           l = (l - n * frequency) - presence
  *   l = l + bias[v];  not allowed: l = -infinity, whatever it was
  * out[r][v] = l.  choice[r] = the lowest index among the largest allowed l (a NaN is larger than everything), -1 where the mask
- * allows no token. */
+ * allows no token.  All three penalties look at the same n: a sampler that counts the prompt for one of them and not for another
+ * is not served.  But for `out` in place, what is written overlaps nothing that the call reads. */
 typedef struct {
   const void* logits;        /* [R][ld] of `dtype`, ld >= V */
   float* out;                /* [R][out_ld], or NULL; may be the logits themselves (fp32, the same pitch) */
